@@ -49,6 +49,7 @@ typedef struct CUstream_st* pto_stream_t; /* cudaStream_t */
 /* dtype of idx_query_scale / idx_key_scale / idx_weight */
 #define PTO_DT_F16 0
 #define PTO_DT_F32 1
+#define PTO_DT_BF16 2 /* rows of the operators around a prompt */
 
 /* flags of the indexer entry points */
 #define PTO_LI_SCORE_SIMT 0x1 /* score stage on CUDA cores (dp4a) instead of tcgen05; validation aid */
@@ -347,6 +348,51 @@ int pto_decode_fused_bf16(const void* idx_query, const void* idx_key_cache, cons
                           int b, int s1, int block_num, int max_blocks, int selected_count, int nq,
                           float softmax_scale, int flags,
                           void* workspace, size_t workspace_bytes, pto_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Operators around a prompt: what a layer does with the rows of a prompt chunk outside the sparse path. They have no
+ * counterpart in the reference's package; rows are bf16 or f16 (`dtype`: PTO_DT_BF16 or PTO_DT_F16), strides are in elements,
+ * every row of a head starts on a 16-byte boundary (strides a multiple of 8).
+ * ------------------------------------------------------------------------------------------ */
+
+/* layouts of the rotated dims: pair i is (x[i], x[i + r/2]); (x[2i], x[2i+1]); or read as the second and written as the first
+ * (what the prologs do to the latent path's rope dims) */
+#define PTO_ROPE_HALF 0
+#define PTO_ROPE_INTERLEAVED 1
+#define PTO_ROPE_DEINTERLEAVE 2
+
+/* RMS norm of every query and key head (where its weight [d] is given) and rotation of `rotary_dim` of its dims (the first ones, or
+ * the last with rope_last) in one pass:
+ *   y = x / sqrt(mean x^2 + eps) * w;   (a, b) -> amplitude * (a cos - b sin, a sin + b cos),  angle = 2 pi position * turns[i] / 2^64
+ *   query [t, hq, dq], key [t, hk, dk] (null with hk = 0), positions int32 (or int64) [t], turns uint64 [rotary_dim/2]
+ *   strides: host array of 8: token and head stride of query, key, query_out, key_out
+ * dq, dk: multiples of 8 up to 256; rotary_dim: a multiple of 16, at most either (0: norm only). An output is its input (in place) or
+ * does not overlap it. */
+int pto_qk_norm_rope(const void* query, const void* key, const void* positions, int positions_int64, const uint64_t* turns,
+                     const void* query_weight, const void* key_weight, void* query_out, void* key_out, int dtype, int t,
+                     int hq, int dq, int hk, int dk, const int64_t* strides, int rotary_dim, int layout, int rope_last,
+                     float amplitude, float eps, pto_stream_t stream);
+
+/* Rows into the quantised paged caches, int8 with one scale per 128 dims (the prologs' arithmetic: q = rint(x * (127 / max)),
+ * scale = 1 / (127 / max)), at row cache_index[i]; rope dims are copied. Index -1: a padding row, not written; another index outside
+ * the cache sets PTO_ST_BAD_PAGE and is skipped. The indices of a call are distinct. Groups below 2^-120 are stored as zeros.
+ *   key_nope [t, width] (row stride ld_nope), width a multiple of 128; key_rope bf16 [t, 64] or null (then rope_cache is not written)
+ *   split caches: nope_cache int8 [cache_rows, width], rope_cache bf16 [cache_rows, 64], scales f32 or f16 [cache_rows, width/128]
+ *   packed_cache int8 [cache_rows, 656] (width 512 with rope); either form may be null
+ * workspace: status words only, PTO_STATUS_WORDS * 4 bytes. */
+int pto_kv_cache_write(const void* key_nope, int64_t ld_nope, const void* key_rope, int64_t ld_rope, const int64_t* cache_index,
+                       int dtype, int t, int width, int8_t* nope_cache, void* rope_cache, void* scales, int scale_dtype,
+                       int8_t* packed_cache, int64_t cache_rows, void* workspace, size_t workspace_bytes, pto_stream_t stream);
+
+/* Positions of sequences back from those caches as contiguous rows: out row cu_seqlens[i] + j = position first[i] + j of sequence i
+ * (first null: 0), for j < cu_seqlens[i+1] - cu_seqlens[i]. Rows behind the last sequence are left as they are; a position without
+ * a valid page is written as zeros and sets PTO_ST_BAD_PAGE.
+ *   block_table int32 [b, max_blocks], cu_seqlens int32 [b+1], nope_out [n, width], rope_out bf16 [n, 64] or null */
+int pto_kv_cache_read(const int8_t* nope_cache, const void* rope_cache, const void* scales, int scale_dtype,
+                      const int8_t* packed_cache, int64_t cache_rows, const int32_t* block_table, const int32_t* cu_seqlens,
+                      const int32_t* first, int b, int max_blocks, int block_size, int64_t n, int width, void* nope_out,
+                      int64_t ld_nope_out, void* rope_out, int64_t ld_rope_out, int dtype, void* workspace,
+                      size_t workspace_bytes, pto_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -13,6 +13,7 @@ _OPS = (
     "mla_indexer_prolog", "decode_indexer_attention_layer",
     "decode_indexer_attention_quant", "workspace_status", "reset_workspace_status", "launch_count",
 )
+_PROMPT = ("RotaryFrequencies", "qk_norm_rope", "kv_cache_write", "kv_cache_read")
 
 
 def __getattr__(name):
@@ -21,4 +22,6 @@ def __getattr__(name):
     # operators resolve lazily so that `pypto_b200.inputs` / `pypto_b200.build` import before the library is built
     if name in _OPS:
         return getattr(importlib.import_module(".ops", __name__), name)
+    if name in _PROMPT:
+        return getattr(importlib.import_module(".prompt", __name__), name)
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -10,7 +10,8 @@ from pathlib import Path
 
 _LIB_PATH = Path(__file__).resolve().parent / "libpypto_b200.so"
 
-PTO_DT_F16, PTO_DT_F32 = 0, 1
+PTO_DT_F16, PTO_DT_F32, PTO_DT_BF16 = 0, 1, 2
+PTO_ROPE_HALF, PTO_ROPE_INTERLEAVED, PTO_ROPE_DEINTERLEAVE = 0, 1, 2
 PTO_LI_SCORE_SIMT, PTO_LI_UNSORTED, PTO_LI_FP16_CHAIN, PTO_LI_EPILOGUE_HIST = 0x1, 0x2, 0x4, 0x8
 PTO_STATUS_WORDS = 8
 PTO_LI_STATIC_SCRATCH_BYTES = (8 << 20) + 256
@@ -49,6 +50,9 @@ SIGNATURES = {
     "pto_decode_workspace_bytes": (_sz, [_i, _i, _i, _i]),
     "pto_decode_fused": (_i, [_vp] * 5 + [_i] + [_vp] * 9 + [_i] * 6 + [_f, _i, _vp, _sz, _vp]),
     "pto_decode_fused_bf16": (_i, [_vp] * 11 + [_i] * 6 + [_f, _i, _vp, _sz, _vp]),
+    "pto_qk_norm_rope": (_i, [_vp] * 3 + [_i] + [_vp] * 5 + [_i] * 6 + [_vp] + [_i] * 3 + [_f, _f, _vp]),
+    "pto_kv_cache_write": (_i, [_vp, _i64, _vp, _i64, _vp] + [_i] * 3 + [_vp] * 3 + [_i, _vp, _i64, _vp, _sz, _vp]),
+    "pto_kv_cache_read": (_i, [_vp] * 3 + [_i, _vp, _i64] + [_vp] * 3 + [_i] * 3 + [_i64, _i, _vp, _i64, _vp, _i64, _i, _vp, _sz, _vp]),
 }
 
 _lib = None

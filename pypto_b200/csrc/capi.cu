@@ -14,6 +14,7 @@
 #include <mutex>
 
 #include "common.cuh"
+#include "rows.cuh"
 
 namespace pto {
 static std::atomic<long long> g_launch_count{0};
@@ -578,6 +579,60 @@ int check_workspace(void* ws, size_t have, size_t need) {
   if (ws == nullptr) return fail(PTO_ERR_WORKSPACE, "workspace is null");
   if ((reinterpret_cast<uintptr_t>(ws) & 255u) != 0) return fail(PTO_ERR_WORKSPACE, "workspace must be 256-byte aligned");
   if (have < need) return fail(PTO_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", have, need);
+  return PTO_OK;
+}
+
+// ---- operators around a prompt -----------------------------------------------------------------------------
+bool row_dtype(int dtype) { return dtype == PTO_DT_BF16 || dtype == PTO_DT_F16; }
+bool row_stride(int64_t s) { return s >= 0 && s % 8 == 0; }  // rows of 16-bit values on 16-byte boundaries
+
+// A tensor [t, heads, d] of norm_rope and its output
+int take_heads(pto::NormRopeSide* s, const char* name, const void* in, void* out, const void* weight, int t, int heads, int d,
+               const int64_t* in_strides, const int64_t* out_strides, int rotary) {
+  PTO_REQUIRE(heads >= 0, "%s: %d heads", name, heads);
+  *s = pto::NormRopeSide{};
+  s->d = 8;
+  if (heads == 0) return PTO_OK;
+  PTO_REQUIRE(in && out, "%s: null tensor pointer", name);
+  PTO_REQUIRE(d >= 8 && d <= 256 && d % 8 == 0, "%s: head of %d dims, a multiple of 8 up to 256 expected", name, d);
+  PTO_REQUIRE(rotary <= d, "%s: %d rotated dims of %d", name, rotary, d);
+  PTO_REQUIRE(aligned16(in) && aligned16(out) && (weight == nullptr || aligned16(weight)), "%s: 16-byte alignment", name);
+  for (int i = 0; i < 2; ++i) {
+    PTO_REQUIRE(row_stride(in_strides[i]) && row_stride(out_strides[i]), "%s: strides must be multiples of 8 elements", name);
+  }
+  PTO_REQUIRE((t == 1 || out_strides[0] >= d) && (heads == 1 || out_strides[1] >= d), "%s: rows of the output overlap", name);
+  PTO_REQUIRE(in != out || (in_strides[0] == out_strides[0] && in_strides[1] == out_strides[1]) || (t == 1 && heads == 1),
+              "%s: output over its input with other strides", name);
+  s->in = in;
+  s->out = out;
+  s->weight = weight;
+  s->in_token = in_strides[0];
+  s->in_head = in_strides[1];
+  s->out_token = out_strides[0];
+  s->out_head = out_strides[1];
+  s->heads = heads;
+  s->d = d;
+  s->rotation_only = in == out && weight == nullptr;
+  return PTO_OK;
+}
+
+// What a write and a read of the quantised caches have in common
+int check_kv(const void* nope, const void* rope, const void* scales, int scale_dtype, const void* packed, int64_t rows, int dtype,
+             int width, bool with_rope) {
+  PTO_REQUIRE(row_dtype(dtype), "dtype %d is neither bf16 nor f16", dtype);
+  PTO_REQUIRE(!with_rope || dtype == PTO_DT_BF16, "rows with rope dims are bf16");
+  PTO_REQUIRE(width >= 128 && width % 128 == 0 && width <= 65536, "width %d: a multiple of 128 up to 65536 expected", width);
+  PTO_REQUIRE(rows >= 1, "cache_rows");
+  PTO_REQUIRE(nope || packed, "null cache pointer");
+  if (nope != nullptr) {
+    PTO_REQUIRE(scales && (rope != nullptr || !with_rope), "null cache pointer");
+    PTO_REQUIRE(scale_dtype == PTO_DT_F16 || scale_dtype == PTO_DT_F32, "scale_dtype %d is neither f16 nor f32", scale_dtype);
+    PTO_REQUIRE(aligned16(nope) && (rope == nullptr || aligned16(rope)), "cache tensors must be 16-byte aligned");
+  }
+  if (packed != nullptr) {
+    PTO_REQUIRE(width == 512 && with_rope, "packed rows are 512 dims and 64 rope dims");
+    PTO_REQUIRE(aligned16(packed), "cache tensors must be 16-byte aligned");
+  }
   return PTO_OK;
 }
 
@@ -1149,6 +1204,110 @@ int pto_decode_fused_bf16(const void* idx_query, const void* idx_key_cache, cons
                  act_seq, attention_out, b, s1, nq, 1, softmax_scale, selected_count, 128,
                  static_cast<int64_t>(block_num) * 128, max_blocks, nq, 0, parts.base, parts.bytes, status, stream,
                  /*behind_topk=*/1);
+}
+
+int pto_qk_norm_rope(const void* query, const void* key, const void* positions, int positions_int64, const uint64_t* turns,
+                     const void* query_weight, const void* key_weight, void* query_out, void* key_out, int dtype, int t,
+                     int hq, int dq, int hk, int dk, const int64_t* strides, int rotary_dim, int layout, int rope_last,
+                     float amplitude, float eps, pto_stream_t stream) {
+  PTO_REQUIRE(row_dtype(dtype), "dtype %d is neither bf16 nor f16", dtype);
+  PTO_REQUIRE(t >= 0, "t %d", t);
+  PTO_REQUIRE(strides != nullptr, "strides is null");
+  PTO_REQUIRE(rotary_dim >= 0 && rotary_dim % 16 == 0, "rotary_dim %d: a multiple of 16 expected", rotary_dim);
+  PTO_REQUIRE(layout >= PTO_ROPE_HALF && layout <= PTO_ROPE_DEINTERLEAVE, "layout %d", layout);
+  if (t == 0 || (hq == 0 && hk == 0)) return PTO_OK;
+  PTO_REQUIRE(rotary_dim == 0 || (positions && turns), "null tensor pointer");
+  pto::NormRopeParams p{};
+  int rc = take_heads(&p.side[0], "query", query, query_out, query_weight, t, hq, dq, strides, strides + 4, rotary_dim);
+  if (rc != PTO_OK) return rc;
+  rc = take_heads(&p.side[1], "key", key, key_out, key_weight, t, hk, dk, strides + 2, strides + 6, rotary_dim);
+  if (rc != PTO_OK) return rc;
+  p.positions = positions;
+  p.positions64 = positions_int64;
+  p.turns = turns;
+  p.amplitude = amplitude;
+  p.eps = eps;
+  p.rotary = rotary_dim;
+  p.rope_last = rope_last;
+  DeviceInfo di;
+  rc = get_device_info(&di);
+  if (rc != PTO_OK) return rc;
+  pto::norm_rope_plan(&p.side[0], t, di.num_sms);
+  pto::norm_rope_plan(&p.side[1], t, di.num_sms);
+  PTO_CUDA(pto::launch_norm_rope(p, dtype, layout, stream));
+  return PTO_OK;
+}
+
+int pto_kv_cache_write(const void* key_nope, int64_t ld_nope, const void* key_rope, int64_t ld_rope, const int64_t* cache_index,
+                       int dtype, int t, int width, int8_t* nope_cache, void* rope_cache, void* scales, int scale_dtype,
+                       int8_t* packed_cache, int64_t cache_rows, void* workspace, size_t workspace_bytes, pto_stream_t stream) {
+  PTO_REQUIRE(t >= 0, "t %d", t);
+  int rc = check_kv(nope_cache, rope_cache, scales, scale_dtype, packed_cache, cache_rows, dtype, width, key_rope != nullptr);
+  if (rc != PTO_OK) return rc;
+  if (t == 0) return PTO_OK;
+  PTO_REQUIRE(key_nope && cache_index, "null tensor pointer");
+  PTO_REQUIRE(aligned16(key_nope) && (key_rope == nullptr || aligned16(key_rope)), "rows must be 16-byte aligned");
+  PTO_REQUIRE(row_stride(ld_nope) && row_stride(ld_rope), "row strides must be multiples of 8 elements");
+  rc = check_workspace(workspace, workspace_bytes, kStatusBytes);
+  if (rc != PTO_OK) return rc;
+  DeviceInfo di;
+  rc = get_device_info(&di);
+  if (rc != PTO_OK) return rc;
+  const int groups = width / 128;
+  const pto::KvWriteParams p{key_nope, key_rope, ld_nope, ld_rope, cache_index, nope_cache, rope_cache, scales, packed_cache,
+                             cache_rows, t, groups, (groups + 3) / 4, scale_dtype == PTO_DT_F16,
+                             reinterpret_cast<int32_t*>(workspace)};
+  PTO_REQUIRE(static_cast<int64_t>(t) * p.chunks <= INT_MAX, "t %d x width %d", t, width);
+  PTO_CUDA(pto::launch_kv_write(p, dtype, stream));
+  return PTO_OK;
+}
+
+int pto_kv_cache_read(const int8_t* nope_cache, const void* rope_cache, const void* scales, int scale_dtype,
+                      const int8_t* packed_cache, int64_t cache_rows, const int32_t* block_table, const int32_t* cu_seqlens,
+                      const int32_t* first, int b, int max_blocks, int block_size, int64_t n, int width, void* nope_out,
+                      int64_t ld_nope_out, void* rope_out, int64_t ld_rope_out, int dtype, void* workspace,
+                      size_t workspace_bytes, pto_stream_t stream) {
+  PTO_REQUIRE(nope_cache == nullptr || packed_cache == nullptr, "two caches to read from");
+  PTO_REQUIRE(b >= 0 && max_blocks >= 0 && block_size >= 1 && n >= 0, "b %d / max_blocks %d / block_size %d / n %lld", b, max_blocks,
+              block_size, static_cast<long long>(n));
+  // (packed rows have rope dims whether or not they are read)
+  int rc = check_kv(nope_cache, rope_cache, scales, scale_dtype, packed_cache, cache_rows, dtype, width,
+                    rope_out != nullptr || packed_cache != nullptr);
+  if (rc != PTO_OK) return rc;
+  if (n == 0 || b == 0) return PTO_OK;
+  PTO_REQUIRE(cu_seqlens && nope_out && (block_table || max_blocks == 0), "null tensor pointer");
+  PTO_REQUIRE(aligned16(nope_out) && (rope_out == nullptr || aligned16(rope_out)), "rows must be 16-byte aligned");
+  PTO_REQUIRE(row_stride(ld_nope_out) && row_stride(ld_rope_out), "row strides must be multiples of 8 elements");
+  PTO_REQUIRE(n == 1 || (ld_nope_out >= width && (rope_out == nullptr || ld_rope_out >= 64)), "rows of the output overlap");
+  PTO_REQUIRE(n <= INT_MAX, "n %lld: cu_seqlens is int32", static_cast<long long>(n));
+  rc = check_workspace(workspace, workspace_bytes, kStatusBytes);
+  if (rc != PTO_OK) return rc;
+  DeviceInfo di;
+  rc = get_device_info(&di);
+  if (rc != PTO_OK) return rc;
+  pto::KvReadParams p{};
+  p.cache = nope_cache;
+  p.rope = rope_cache;
+  p.scales = scales;
+  p.packed = packed_cache;
+  p.table = block_table;
+  p.cu = cu_seqlens;
+  p.first = first;
+  p.out = nope_out;
+  p.rope_out = rope_out;
+  p.out_ld = ld_nope_out;
+  p.rope_out_ld = ld_rope_out;
+  p.rows = cache_rows;
+  p.n = n;
+  p.b = b;
+  p.max_blocks = max_blocks;
+  p.block_size = block_size;
+  p.groups = width / 128;
+  p.chunks = (p.groups + 3) / 4;
+  p.scale_f16 = scale_dtype == PTO_DT_F16;
+  p.status = reinterpret_cast<int32_t*>(workspace);
+  PTO_CUDA(pto::launch_kv_read(p, dtype, di.num_sms, stream));
+  return PTO_OK;
 }
 
 }  // extern "C"
