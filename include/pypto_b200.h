@@ -67,7 +67,7 @@ typedef struct CUstream_st* pto_stream_t; /* cudaStream_t */
 
 /* device status area at the start of every workspace */
 #define PTO_STATUS_WORDS 8
-#define PTO_ST_BAD_PAGE 0x1    /* a block-table entry or top-k index outside its range was skipped */
+#define PTO_ST_BAD_PAGE 0x1    /* a block-table entry, top-k index, cache index or sequence offset outside its range was skipped */
 #define PTO_ST_WAIT_EXPIRED 0x2 /* a bounded mbarrier wait gave up; results are incomplete */
 /* word 3 counts the rows whose selection fell back to the radix select (massive ties, values that are not
  * finite): right, but several scans of the row by one SM. Not an error. */
@@ -393,6 +393,23 @@ int pto_kv_cache_read(const int8_t* nope_cache, const void* rope_cache, const vo
                       const int32_t* first, int b, int max_blocks, int block_size, int64_t n, int width, void* nope_out,
                       int64_t ld_nope_out, void* rope_out, int64_t ld_rope_out, int dtype, void* workspace,
                       size_t workspace_bytes, pto_stream_t stream);
+
+/* Attention over packed prompts: token i of a sequence's lq sees keys j <= i + lk - lq of its lk (all of them without `causal`).
+ *   out_i = sum_j softmax_j(softmax_scale * q_i . k_j) v_j;   lse = ln sum_j exp(softmax_scale * q_i . k_j)
+ * A token that sees no key gets zeros and lse -inf. Query head h reads key head h / (hq / hkv).
+ *   query [tq, hq, dqk], key [tk, hkv, dqk], value [tk, hkv, dv], attention_out [tq, hq, dv], lse_out f32 [hq, tq] or NULL;
+ *   (dqk, dv): (64, 64), (128, 128), (192, 128); hq a multiple of hkv
+ *   cu_seqlens_q, cu_seqlens_k int32 [b+1]: where the sequences begin, from 0, not decreasing, the last entry where the last ends.
+ *   Rows behind it are left as they are. Offsets out of order or range set PTO_ST_BAD_PAGE and reach nothing outside the tensors.
+ *   strides: host array of 8: token and head stride of query, key, value, attention_out
+ * Scores, sums and outputs are fp32, probabilities are rounded to the rows' type before they are multiplied with the values. What a
+ * token does not see does not reach its result, whatever it holds. Deterministic: the same call gives the same bits. */
+size_t pto_prompt_attention_workspace_bytes(int tq, int tk, int b, int hq, int hkv, int dv);
+
+int pto_prompt_attention(const void* query, const void* key, const void* value, const int32_t* cu_seqlens_q,
+                         const int32_t* cu_seqlens_k, void* attention_out, float* lse_out, int dtype, int tq, int tk, int b, int hq,
+                         int hkv, int dqk, int dv, const int64_t* strides, float softmax_scale, int causal, void* workspace,
+                         size_t workspace_bytes, pto_stream_t stream);
 
 #ifdef __cplusplus
 }

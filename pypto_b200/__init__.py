@@ -13,7 +13,7 @@ _OPS = (
     "mla_indexer_prolog", "decode_indexer_attention_layer",
     "decode_indexer_attention_quant", "workspace_status", "reset_workspace_status", "launch_count",
 )
-_PROMPT = ("RotaryFrequencies", "qk_norm_rope", "kv_cache_write", "kv_cache_read")
+_PROMPT = ("RotaryFrequencies", "qk_norm_rope", "kv_cache_write", "kv_cache_read", "prompt_attention")
 
 
 def __getattr__(name):

@@ -50,6 +50,8 @@ SIGNATURES = {
     "pto_decode_workspace_bytes": (_sz, [_i, _i, _i, _i]),
     "pto_decode_fused": (_i, [_vp] * 5 + [_i] + [_vp] * 9 + [_i] * 6 + [_f, _i, _vp, _sz, _vp]),
     "pto_decode_fused_bf16": (_i, [_vp] * 11 + [_i] * 6 + [_f, _i, _vp, _sz, _vp]),
+    "pto_prompt_attention_workspace_bytes": (_sz, [_i] * 6),
+    "pto_prompt_attention": (_i, [_vp] * 7 + [_i] * 8 + [_vp, _f, _i, _vp, _sz, _vp]),
     "pto_qk_norm_rope": (_i, [_vp] * 3 + [_i] + [_vp] * 5 + [_i] * 6 + [_vp] + [_i] * 3 + [_f, _f, _vp]),
     "pto_kv_cache_write": (_i, [_vp, _i64, _vp, _i64, _vp] + [_i] * 3 + [_vp] * 3 + [_i, _vp, _i64, _vp, _sz, _vp]),
     "pto_kv_cache_read": (_i, [_vp] * 3 + [_i, _vp, _i64] + [_vp] * 3 + [_i] * 3 + [_i64, _i, _vp, _i64, _vp, _i64, _i, _vp, _sz, _vp]),

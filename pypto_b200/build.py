@@ -17,8 +17,8 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libpypto_b200.so"
 SOURCES = ["capi.cu", "li_score.cu", "topk_select.cu", "sfa_decode.cu", "sfa_pair.cu", "sfa_slice.cu", "prolog.cu", "prolog_gemm.cu",
-           "prolog_sgemm.cu", "prolog_wide.cu", "rows.cu"]
-HEADERS = [CSRC / "common.cuh", CSRC / "sfa_common.cuh", CSRC / "rows.cuh", PKG.parent / "include" / "pypto_b200.h"]
+           "prolog_sgemm.cu", "prolog_wide.cu", "rows.cu", "prompt_attention.cu"]
+HEADERS = [CSRC / "common.cuh", CSRC / "sfa_common.cuh", CSRC / "rows.cuh", CSRC / "prompt_attention.cuh", PKG.parent / "include" / "pypto_b200.h"]
 
 
 NATIVE = PKG / "_native.so"

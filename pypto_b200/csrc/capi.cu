@@ -14,6 +14,7 @@
 #include <mutex>
 
 #include "common.cuh"
+#include "prompt_attention.cuh"
 #include "rows.cuh"
 
 namespace pto {
@@ -614,6 +615,53 @@ int take_heads(pto::NormRopeSide* s, const char* name, const void* in, void* out
   s->d = d;
   s->rotation_only = in == out && weight == nullptr;
   return PTO_OK;
+}
+
+// 3-D map over rows [tokens, heads, dims] of 16-bit values, boxes of 128 tokens x one head x 64 dims, 128-byte swizzle
+int make_heads_map(CUtensorMap* map, const void* base, int tokens, int heads, int dims, int64_t token_stride, int64_t head_stride) {
+  EncodeTiledFn enc;
+  int rc = get_encode_fn(&enc);
+  if (rc != PTO_OK) return rc;
+  // (a dim of one is never stepped along; the driver wants a stride all the same)
+  const int64_t hs = heads > 1 ? head_stride : dims, ts = tokens > 1 ? token_stride : dims;
+  cuuint64_t dim[3] = {static_cast<cuuint64_t>(dims), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(tokens)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(hs) * 2, static_cast<cuuint64_t>(ts) * 2};
+  cuuint32_t box[3] = {64, 1, 128};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), dim, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(PTO_ERR_DRIVER, "cuTensorMapEncodeTiled failed with %d", static_cast<int>(r));
+  return PTO_OK;
+}
+
+// Workspace of the prompt attention: status, tables, partial results
+struct PaWs {
+  bool self_plan;
+  int max_tiles, slot_rows, slots;
+  int64_t table_stride;
+  size_t tables, part_ml, part_o, total;
+};
+PaWs pa_ws(int tq, int tk, int b, int hq, int hkv, int dv) {
+  PaWs w{};
+  const int group = hq / hkv;
+  const int64_t rows = static_cast<int64_t>(tq) * group;  // of a key head
+  w.max_tiles = static_cast<int>(rows / pto::kPaRows + b);
+  w.self_plan = w.max_tiles <= pto::kPaSmallTiles;
+  w.table_stride = static_cast<int64_t>(
+      align_up(sizeof(pto::PaHead) + sizeof(pto::PaTile) * static_cast<size_t>(w.max_tiles) + sizeof(int) * (static_cast<size_t>(b) + 1), 256));
+  w.slot_rows = static_cast<int>(rows < pto::kPaRows ? rows : pto::kPaRows);
+  const int64_t longest = (static_cast<int64_t>(tk) + pto::kPaKeys - 1) / pto::kPaKeys;  // key tiles of an item
+  if (longest > pto::kPaMinPiece) {
+    const int64_t all = (longest + pto::kPaMinPiece - 1) / pto::kPaMinPiece * w.max_tiles * hkv;
+    w.slots = static_cast<int>(all < pto::kPaSlots ? all : pto::kPaSlots);
+  }
+  w.tables = kStatusBytes;
+  w.part_ml = w.tables + static_cast<size_t>(w.table_stride) * (w.self_plan ? pto::kPaCtas : 1);
+  const size_t part_rows = static_cast<size_t>(w.slots) * w.slot_rows;
+  w.part_o = w.part_ml + align_up(part_rows * sizeof(float2), 256);
+  w.total = w.part_o + align_up(part_rows * dv * sizeof(float), 256);
+  return w;
 }
 
 // What a write and a read of the quantised caches have in common
@@ -1307,6 +1355,95 @@ int pto_kv_cache_read(const int8_t* nope_cache, const void* rope_cache, const vo
   p.scale_f16 = scale_dtype == PTO_DT_F16;
   p.status = reinterpret_cast<int32_t*>(workspace);
   PTO_CUDA(pto::launch_kv_read(p, dtype, di.num_sms, stream));
+  return PTO_OK;
+}
+
+size_t pto_prompt_attention_workspace_bytes(int tq, int tk, int b, int hq, int hkv, int dv) {
+  if (tq < 0 || tk < 0 || b < 1 || hkv < 1 || hq < hkv || dv < 1 || static_cast<int64_t>(tq) * (hq / hkv) > INT_MAX - 512) return 0;
+  return pa_ws(tq, tk, b, hq, hkv, dv).total;
+}
+
+int pto_prompt_attention(const void* query, const void* key, const void* value, const int32_t* cu_seqlens_q,
+                         const int32_t* cu_seqlens_k, void* attention_out, float* lse_out, int dtype, int tq, int tk, int b, int hq,
+                         int hkv, int dqk, int dv, const int64_t* strides, float softmax_scale, int causal, void* workspace,
+                         size_t workspace_bytes, pto_stream_t stream) {
+  PTO_REQUIRE(row_dtype(dtype), "dtype %d is neither bf16 nor f16", dtype);
+  PTO_REQUIRE((dqk == 64 && dv == 64) || (dqk == 128 && dv == 128) || (dqk == 192 && dv == 128),
+              "head dims %d / %d: 64 / 64, 128 / 128 or 192 / 128 expected", dqk, dv);
+  PTO_REQUIRE(tq >= 0 && tk >= 0 && b >= 0, "tq %d / tk %d / b %d", tq, tk, b);
+  PTO_REQUIRE(hkv >= 1 && hq >= hkv && hq % hkv == 0, "%d query heads of %d key heads", hq, hkv);
+  PTO_REQUIRE(softmax_scale > 0.f && softmax_scale <= 1e30f, "softmax_scale must be positive and finite");
+  PTO_REQUIRE(strides != nullptr, "strides is null");
+  if (tq == 0 || b == 0) return PTO_OK;
+  const int group = hq / hkv;
+  PTO_REQUIRE(query && attention_out && cu_seqlens_q && cu_seqlens_k && (tk == 0 || (key && value)), "null tensor pointer");
+  PTO_REQUIRE(aligned16(query) && aligned16(attention_out) && aligned16(key) && aligned16(value), "rows must be 16-byte aligned");
+  for (int i = 0; i < 8; ++i) PTO_REQUIRE(row_stride(strides[i]), "strides must be multiples of 8 elements");
+  const int width[4] = {dqk, dqk, dv, dv}, tokens[4] = {tq, tk, tk, tq}, heads[4] = {hq, hkv, hkv, hq};
+  for (int i = 1; i < 4; ++i) {  // (queries may be the same row more than once)
+    PTO_REQUIRE((tokens[i] <= 1 || strides[2 * i] >= width[i]) && (heads[i] <= 1 || strides[2 * i + 1] >= width[i]),
+                "rows of the keys, values or output overlap");
+    PTO_REQUIRE(strides[2 * i] < (1ll << 38) && strides[2 * i + 1] < (1ll << 38), "strides");
+  }
+  PTO_REQUIRE(static_cast<int64_t>(tq) * group <= INT_MAX - 512 && tk <= INT_MAX - 512, "tq %d x %d heads / tk %d", tq, group, tk);
+  const PaWs w = pa_ws(tq, tk, b, hq, hkv, dv);
+  PTO_REQUIRE((static_cast<int64_t>(w.max_tiles) + pto::kPaSlots) * hkv < INT_MAX / 2, "too many work items");
+  int rc = check_workspace(workspace, workspace_bytes, w.total);
+  if (rc != PTO_OK) return rc;
+  DeviceInfo di;
+  rc = get_device_info(&di);
+  if (rc != PTO_OK) return rc;
+  alignas(64) CUtensorMap map_k, map_v;
+  memset(&map_k, 0, sizeof(map_k));
+  memset(&map_v, 0, sizeof(map_v));
+  if (tk > 0) {
+    rc = make_heads_map(&map_k, key, tk, hkv, dqk, strides[2], strides[3]);
+    if (rc != PTO_OK) return rc;
+    rc = make_heads_map(&map_v, value, tk, hkv, dv, strides[4], strides[5]);
+    if (rc != PTO_OK) return rc;
+  }
+  uint8_t* base = reinterpret_cast<uint8_t*>(workspace);
+  pto::PaParams p{};
+  p.q = query;
+  p.out = attention_out;
+  p.v = value;
+  p.lse = lse_out;
+  p.q_token = strides[0];
+  p.q_head = strides[1];
+  p.v_token = strides[4];
+  p.v_head = strides[5];
+  p.out_token = strides[6];
+  p.out_head = strides[7];
+  p.cu_q = cu_seqlens_q;
+  p.cu_k = cu_seqlens_k;
+  p.tq = tq;
+  p.tk = tk;
+  p.b = b;
+  p.hq = hq;
+  p.hkv = hkv;
+  p.group = group;
+  int l = 0;
+  while ((1ll << l) < group) ++l;
+  p.group_shift = 31 + l;
+  p.group_mul = static_cast<uint32_t>((1ull << p.group_shift) / static_cast<uint32_t>(group) + 1);
+  p.causal = causal != 0;
+  // key heads worked on together: as many as half of L2 holds the keys and values of
+  const int64_t head_bytes = static_cast<int64_t>(tk) * (dqk + dv) * 2;
+  const int64_t set = head_bytes > 0 ? (64ll << 20) / head_bytes : hkv;
+  p.head_set = static_cast<int>(set < 1 ? 1 : set > hkv ? hkv : set);
+  p.scale = softmax_scale;
+  p.scale_log2 = softmax_scale * 1.44269504088896340736f;
+  p.max_tiles = w.max_tiles;
+  p.slot_rows = w.slot_rows;
+  p.self_plan = w.self_plan;
+  p.tables = base + w.tables;
+  p.table_stride = w.table_stride;
+  p.part_ml = reinterpret_cast<float2*>(base + w.part_ml);
+  p.part_o = reinterpret_cast<float*>(base + w.part_o);
+  p.slots = w.slots;
+  p.status = reinterpret_cast<int32_t*>(workspace);
+  const int ctas = di.num_sms < pto::kPaCtas ? di.num_sms : pto::kPaCtas;
+  PTO_CUDA(pto::launch_prompt_attention(p, dqk, dv, dtype, &map_k, &map_v, ctas, stream));
   return PTO_OK;
 }
 

@@ -3,6 +3,7 @@
   qk_norm_rope        RMS norm of every query and key head and rotation of part of the head, one pass
   kv_cache_write      rows into the quantised paged caches (split arrays, packed rows)
   kv_cache_read       positions of sequences back from those caches as contiguous rows
+  prompt_attention    dense causal attention of packed sequences with grouped heads
 
 They take raw torch tensors or `from_torch` handles on one CUDA device, write their outputs in place, return None and run
 asynchronously on the current stream, as the operators of `ops`. Rows are bfloat16 or float16. Unlike there, tensors of rows may be
@@ -265,4 +266,47 @@ def kv_cache_read(key_nope_2d, key_rope_2d, k_nope_scales, block_table, cu_seqle
             int(block_size), n, width, out.data_ptr(), _stride(out, 0), ro.data_ptr() if ro is not None else None,
             _stride(ro, 0) if ro is not None else 0, _ROW_DTYPES[out.dtype], ws.data_ptr(), ws.numel(),
             torch.cuda.current_stream(dev).cuda_stream))
+    return None
+
+
+def prompt_attention(query, key, value, cu_seqlens_q, cu_seqlens_k, attention_out, softmax_scale=None, *, causal=True, lse_out=None):
+    """Attention of packed sequences over all of their keys: token i of a sequence's lq sees keys j <= i + lk - lq of its lk (all of
+    them with causal=False), so a chunk of a prompt comes with its earlier keys in front, and a single token with its whole context.
+
+    query [tq, hq, dqk], key [tk, hkv, dqk], value [tk, hkv, dv], attention_out [tq, hq, dv]; (dqk, dv) (64, 64), (128, 128) or
+    (192, 128) (the latent path after its up-projections); query head h reads key head h / (hq / hkv). cu_seqlens_q, cu_seqlens_k int32
+    [b + 1]: where the sequences begin, from 0, not decreasing; rows of the output behind the last sequence are left as they are.
+    softmax_scale positive, by default dqk^-0.5. `lse_out` (float32 [hq, tq], optional) receives ln sum exp of the scaled scores, with
+    which results over different keys can be joined. A token without a key gets zeros and -inf."""
+    q, k, v, out = _rows(query, "query", 3), _rows(key, "key", 3), _rows(value, "value", 3), _rows(attention_out, "attention_out", 3)
+    tq, hq, dqk = q.shape
+    tk, hkv, dv = v.shape
+    _need(tuple(k.shape) == (tk, hkv, dqk), "key: [tk, hkv, dqk] beside value [tk, hkv, dv]")
+    _need((dqk, dv) in ((64, 64), (128, 128), (192, 128)), f"head dims {dqk} / {dv}: 64 / 64, 128 / 128 or 192 / 128 expected")
+    _need(hkv >= 1 and hq >= 1 and hq % hkv == 0, "query heads must be a multiple of the key heads")
+    _need(tuple(out.shape) == (tq, hq, dv), "attention_out: [tq, hq, dv]")
+    _need(q.dtype == k.dtype == v.dtype == out.dtype, "query, key, value and attention_out must share one dtype")
+    cq, ck = unwrap(cu_seqlens_q, "cu_seqlens_q"), unwrap(cu_seqlens_k, "cu_seqlens_k")
+    _need(cq.dtype == ck.dtype == torch.int32 and cq.dim() == 1 and cq.shape[0] >= 1 and cq.shape == ck.shape,
+          "cu_seqlens_q, cu_seqlens_k: int32 [b + 1]")
+    scale = dqk ** -0.5 if softmax_scale is None else float(softmax_scale)
+    _need(0.0 < scale <= 1e30, "softmax_scale must be positive and finite")
+    tensors, lse = [q, k, v, out, cq, ck], None
+    if lse_out is not None:
+        lse = unwrap(lse_out, "lse_out")
+        _need(lse.dtype == torch.float32 and tuple(lse.shape) == (hq, tq), "lse_out: float32 [hq, tq]")
+        tensors.append(lse)
+    dev = _same_device(tensors)
+    b = cq.shape[0] - 1
+    if tq == 0 or b == 0:
+        return None
+    lib = _lib.load()
+    nbytes = lib.pto_prompt_attention_workspace_bytes(tq, tk, b, hq, hkv, dv)
+    strides = (C.c_int64 * 8)(*[_stride(x, i) for x in (q, k, v, out) for i in (0, 1)])
+    with torch.cuda.device(dev):
+        ws = _workspace(dev, max(nbytes, 256))
+        _lib.check(lib.pto_prompt_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), cq.data_ptr(), ck.data_ptr(), out.data_ptr(),
+                                            lse.data_ptr() if lse is not None else None, _ROW_DTYPES[q.dtype], tq, tk, b, hq, hkv,
+                                            dqk, dv, strides, scale, int(bool(causal)), ws.data_ptr(), ws.numel(),
+                                            torch.cuda.current_stream(dev).cuda_stream))
     return None

@@ -96,8 +96,54 @@ def test_cache_read_refuses(over, exc):
         pto.kv_cache_read(**read(**over))
 
 
+def prompt(**over):
+    a = dict(query=torch.zeros(5, 4, 128, dtype=BF), key=torch.zeros(9, 2, 128, dtype=BF), value=torch.zeros(9, 2, 128, dtype=BF),
+             cu_seqlens_q=torch.tensor([0, 2, 5], dtype=torch.int32), cu_seqlens_k=torch.tensor([0, 4, 9], dtype=torch.int32),
+             attention_out=torch.zeros(5, 4, 128, dtype=BF))
+    a.update(over)
+    return a
+
+
+@pytest.mark.parametrize("over,exc", [
+    ({}, RuntimeError),
+    (dict(query=torch.zeros(5, 3, 128, dtype=BF), attention_out=torch.zeros(5, 3, 128, dtype=BF)), ValueError),  # heads
+    (dict(query=torch.zeros(5, 4, 96, dtype=BF)), ValueError),
+    (dict(key=torch.zeros(9, 2, 64, dtype=BF)), ValueError),
+    (dict(value=torch.zeros(8, 2, 128, dtype=BF)), ValueError),
+    (dict(value=torch.zeros(9, 2, 64, dtype=BF), attention_out=torch.zeros(5, 4, 64, dtype=BF)), ValueError),
+    (dict(key=torch.zeros(9, 2, 128, dtype=torch.float16)), ValueError),
+    (dict(query=torch.zeros(5, 4, 128)), ValueError),
+    (dict(attention_out=torch.zeros(5, 4, 64, dtype=BF)), ValueError),
+    (dict(cu_seqlens_q=torch.tensor([0, 2, 5])), ValueError),
+    (dict(cu_seqlens_k=torch.tensor([0, 9], dtype=torch.int32)), ValueError),
+    (dict(softmax_scale=0.0), ValueError),
+    (dict(softmax_scale=-1.0), ValueError),
+    (dict(softmax_scale=math.nan), ValueError),
+    (dict(lse_out=torch.zeros(5, 4)), ValueError),
+    (dict(lse_out=torch.zeros(4, 5, dtype=BF)), ValueError),
+    (dict(query=torch.zeros(4, 5, 136, dtype=BF).transpose(0, 1)[..., 4:132]), ValueError),  # off 16-byte boundaries
+    (dict(key=None), TypeError),
+])
+def test_prompt_attention_refuses(over, exc):
+    with pytest.raises(exc):
+        pto.prompt_attention(**prompt(**over))
+
+
+def test_prompt_attention_workspace():
+    lib = _lib.load()
+    # short contexts are never cut into pieces: status words and tables only
+    assert lib.pto_prompt_attention_workspace_bytes(17, 17, 1, 8, 2, 64) < 1 << 20
+    # the pieces of one token's context: at most 8 x 148 of the group's rows
+    one = lib.pto_prompt_attention_workspace_bytes(1, 1 << 20, 1, 8, 1, 128)
+    assert 0 < one < (1 << 20) + 8 * 148 * 8 * 130 * 4
+    assert lib.pto_prompt_attention_workspace_bytes(1 << 17, 1 << 17, 4, 128, 8, 128) < 200 << 20
+    assert lib.pto_prompt_attention_workspace_bytes(1, 1, 0, 1, 1, 64) == 0
+
+
 def test_c_entries_refuse_before_any_cuda_call():
     lib = _lib.load()
+    assert lib.pto_prompt_attention(None, None, None, None, None, None, None, 2, 1, 1, 1, 1, 1, 64, 64, None, 1.0, 1, None, 0,
+                                    None) == -1
     assert lib.pto_qk_norm_rope(None, None, None, 0, None, None, None, None, None, 2, 1, 1, 64, 0, 64, None, 0, 0, 0, 1.0, 1e-6,
                                 None) == -1
     assert lib.pto_kv_cache_write(None, 512, None, 0, None, 2, 1, 512, None, None, None, 1, None, 128, None, 0, None) == -1
