@@ -617,8 +617,9 @@ int take_heads(pto::NormRopeSide* s, const char* name, const void* in, void* out
   return PTO_OK;
 }
 
-// 3-D map over rows [tokens, heads, dims] of 16-bit values, boxes of 128 tokens x one head x 64 dims, 128-byte swizzle
-int make_heads_map(CUtensorMap* map, const void* base, int tokens, int heads, int dims, int64_t token_stride, int64_t head_stride) {
+// 3-D map over rows [tokens, heads, dims] of 16-bit values, boxes of 128 rows (128 / box_heads tokens) x 64 dims, 128-byte swizzle
+int make_heads_map(CUtensorMap* map, const void* base, int tokens, int heads, int dims, int64_t token_stride, int64_t head_stride,
+                   int box_heads = 1) {
   EncodeTiledFn enc;
   int rc = get_encode_fn(&enc);
   if (rc != PTO_OK) return rc;
@@ -626,7 +627,7 @@ int make_heads_map(CUtensorMap* map, const void* base, int tokens, int heads, in
   const int64_t hs = heads > 1 ? head_stride : dims, ts = tokens > 1 ? token_stride : dims;
   cuuint64_t dim[3] = {static_cast<cuuint64_t>(dims), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(tokens)};
   cuuint64_t strides[2] = {static_cast<cuuint64_t>(hs) * 2, static_cast<cuuint64_t>(ts) * 2};
-  cuuint32_t box[3] = {64, 1, 128};
+  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(128 / box_heads)};
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), dim, strides, box, estr,
                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -647,7 +648,8 @@ PaWs pa_ws(int tq, int tk, int b, int hq, int hkv, int dv) {
   const int group = hq / hkv;
   const int64_t rows = static_cast<int64_t>(tq) * group;  // of a key head
   w.max_tiles = static_cast<int>(rows / pto::kPaRows + b);
-  w.self_plan = w.max_tiles <= pto::kPaSmallTiles;
+  // one wave of items: every CTA finds its own; more are handed out as CTAs become free, from a table made by a kernel in front
+  w.self_plan = w.max_tiles <= pto::kPaSmallTiles && static_cast<int64_t>(w.max_tiles) * hkv <= pto::kPaCtas;
   w.table_stride = static_cast<int64_t>(
       align_up(sizeof(pto::PaHead) + sizeof(pto::PaTile) * static_cast<size_t>(w.max_tiles) + sizeof(int) * (static_cast<size_t>(b) + 1), 256));
   w.slot_rows = static_cast<int>(rows < pto::kPaRows ? rows : pto::kPaRows);
@@ -1393,7 +1395,8 @@ int pto_prompt_attention(const void* query, const void* key, const void* value, 
   DeviceInfo di;
   rc = get_device_info(&di);
   if (rc != PTO_OK) return rc;
-  alignas(64) CUtensorMap map_k, map_v;
+  alignas(64) CUtensorMap map_q, map_k, map_v;
+  memset(&map_q, 0, sizeof(map_q));
   memset(&map_k, 0, sizeof(map_k));
   memset(&map_v, 0, sizeof(map_v));
   if (tk > 0) {
@@ -1402,8 +1405,14 @@ int pto_prompt_attention(const void* query, const void* key, const void* value, 
     rc = make_heads_map(&map_v, value, tk, hkv, dv, strides[4], strides[5]);
     if (rc != PTO_OK) return rc;
   }
-  uint8_t* base = reinterpret_cast<uint8_t*>(workspace);
   pto::PaParams p{};
+  // (rows that lie apart: a stride of 0, one query row for several heads, is no tensor map's)
+  p.q_map = 128 % group == 0 && (tq == 1 || strides[0] > 0) && (hq == 1 || strides[1] > 0) && strides[0] < (1ll << 38) && strides[1] < (1ll << 38);
+  if (p.q_map) {
+    rc = make_heads_map(&map_q, query, tq, hq, dqk, strides[0], strides[1], group);
+    if (rc != PTO_OK) return rc;
+  }
+  uint8_t* base = reinterpret_cast<uint8_t*>(workspace);
   p.q = query;
   p.out = attention_out;
   p.v = value;
@@ -1443,7 +1452,7 @@ int pto_prompt_attention(const void* query, const void* key, const void* value, 
   p.slots = w.slots;
   p.status = reinterpret_cast<int32_t*>(workspace);
   const int ctas = di.num_sms < pto::kPaCtas ? di.num_sms : pto::kPaCtas;
-  PTO_CUDA(pto::launch_prompt_attention(p, dqk, dv, dtype, &map_k, &map_v, ctas, stream));
+  PTO_CUDA(pto::launch_prompt_attention(p, dqk, dv, dtype, &map_q, &map_k, &map_v, ctas, stream));
   return PTO_OK;
 }
 

@@ -2,14 +2,17 @@
 // pass over the keys with a running maximum and sum.
 //
 // The query heads of a key head are rows of one matrix (row = token * group + head), so a work item is 256 rows of a sequence
-// against its keys: two MMA tiles of 128 rows, and every K and V tile that is loaded serves both. TMEM holds the scores of both
-// tiles (2 x 128 columns) and both outputs (2 x dv); probabilities overwrite their scores as 16-bit values and are the A operand
-// of the value product from there. While the softmax of one tile runs, the tensor pipe works for the other:
-//   S0(0) S1(0) | PV0(0) S0(1) PV1(0) S1(1) | PV0(1) S0(2) ...
+// against its keys: two MMA tiles of 128 rows, two streams, and every K and V tile that is loaded serves both. A stream goes in
+// steps of 64 keys. TMEM holds the scores of two steps of each stream, whose first half the probabilities overwrite as 16-bit
+// values (the A operand of the value product from there), and both outputs; the scores of step i + 2 follow the value product of
+// step i, so the softmax finds the next step's scores ready while the tensor pipe works on the ones before. (Steps of 128 keys
+// in one buffer: the pipe waited for the softmax and the softmax for it, 8192 tokens x 32 heads 490 us; in buffers of their own for
+// scores and probabilities, two hand-overs a step, 505. Score products of 64 keys take the pipe 48 cycles instead of 32: shared
+// memory delivers 128 bytes a cycle.)
 // An item of at most 128 rows (a few tokens, single ones) has one tile; both streams take it, each with half of the keys, and the
 // halves are merged at the end.
-// Warps: 0 issues MMAs, 1 hands out items and loads K and V by TMA through a ring, 2 and 3 load queries and mend the value tiles at
-// a mask's edge, 4-7 and 8-11 are the softmax of stream 0 and 1, one thread a row.
+// Warps: 0 and 1 issue the MMAs of stream 0 and 1, 2 hands out items and loads K and V by TMA through a ring, 3 loads queries and
+// mends the value tiles at a mask's edge, 4-7 and 8-11 are the softmax of stream 0 and 1, one thread a row.
 #include "prompt_attention.cuh"
 #include "sfa_common.cuh"
 
@@ -28,11 +31,14 @@ struct Cfg {
   static constexpr int kQ = DQK / 64 * kBox;
   static constexpr int kRing = (14 * kBox - 2 * kQ) / kSlot;  // 12, 5, 8 slots
   static constexpr int kK = DQK / 64 / kSlotBoxes, kV = DV / 64 / kSlotBoxes;  // slots of a K and of a V tile
+  static constexpr int kStep = 64, kSteps = kPaKeys / kStep;  // keys of a step, steps of a tile
+  static constexpr uint32_t kColO = 256;                      // first column of the outputs, behind two streams' two buffers of scores
   static constexpr uint32_t kFmt = F16 ? 0u : kABFmtBF16;
   static constexpr uint32_t kNonFinite = F16 ? 0x7c00u : 0x7f80u;  // exponent bits
   // f16 probabilities are kept away from its subnormal values: times 2^4 (a maximum that lags by 2^8 leaves them below 2^12)
   static constexpr float kBias = F16 ? 4.f : 0.f;
 };
+constexpr int kFmaPairs = 0;  // of eight pairs of probabilities, those whose exponentials the FMA pipe computes
 constexpr float kLag = 8.f;  // a maximum is raised, and the output rescaled, once it is 2^8 behind
 
 struct Item {
@@ -40,6 +46,7 @@ struct Item {
   int q0, row0, rows;        // first token of the sequence, first row, rows of the item
   int k0, lk, seen;          // first key, keys; row r sees min(lk, seen + token) keys
   int begin[2], end[2];      // key tiles of the two streams
+  int last[2];               // keys that some row of a stream sees
   int edge, keys;            // keys from `edge` on are hidden from some row, from `keys` on from all of them
   int head, slot;            // key head; slot of the partial result, -1: the item is whole
 };
@@ -47,11 +54,11 @@ struct Item {
 constexpr int kMaxRing = 12;
 struct Ctl {
   unsigned long long full[kMaxRing], raw[kMaxRing], empty[kMaxRing];
-  unsigned long long qfull[2], qempty, sfull[2], pfull[2], ofull[2], xfull, xempty, mfull[2], mempty[2], drain;
+  unsigned long long qfull[2], qempty, sfull[2][2], pfull[2][2], pfree[2], ofull[2], xfull, xempty, mfull[2], mempty[2], drain[2];
   Item item[2];
-  int odd[2][2];  // values that are not finite were taken out of an item's tiles (by warp 2, by warp 3)
+  int odd[2];  // values that are not finite were taken out of an item's tiles
   uint32_t tmem;
-  int scan[32];
+  int expired;
   float2 xch[128];  // maximum and sum of stream 1
 };
 static_assert(sizeof(Ctl) <= 2048, "control block");
@@ -62,15 +69,32 @@ struct Ctx {
   uint32_t q, ring, tmem;
 };
 
-__device__ __forceinline__ bool wait_bar(const unsigned long long& bar, uint32_t parity, int32_t* status, int site) {
-  if (mbar_wait_spin(smem_u32(&bar), parity)) return true;
-  set_status(status, PTO_ST_WAIT_EXPIRED, site, site);
-  return false;
+// Waits for a phase. A wait that runs out sets the status and `expired`, after which no wait of the CTA waits any more and nothing
+// more is loaded: the loops run to their ends on whatever is there. One test, without a vote, is all that a phase that is
+// complete costs; callers of warp-wide instructions converge behind it.
+__device__ __forceinline__ void wait_bar(Ctl* c, uint32_t bar, uint32_t parity, int32_t* status, int site) {
+  if (mbar_try_wait(bar, parity)) return;
+  const long long t0 = clock64();
+#pragma unroll 1
+  while (!mbar_try_wait(bar, parity)) {
+    if (*reinterpret_cast<volatile int*>(&c->expired)) return;
+    if (clock64() - t0 > kWaitBudgetCycles) {
+      c->expired = 1;
+      set_status(status, PTO_ST_WAIT_EXPIRED, site, site);
+      return;
+    }
+  }
 }
-__device__ __forceinline__ bool wait_warp(const unsigned long long& bar, uint32_t parity, int32_t* status, int site) {
-  return __all_sync(0xffffffffu, wait_bar(bar, parity, status, site));
+__device__ __forceinline__ void wait_warp(Ctl* c, unsigned long long& bar, uint32_t parity, int32_t* status, int site) {
+  wait_bar(c, smem_u32(&bar), parity, status, site);
+  __syncwarp();
 }
 
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* map, int x, int y, int z, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+               "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+               : "memory");
+}
 __device__ __forceinline__ int row_token(const PaParams& p, int row) {
   return static_cast<int>((static_cast<unsigned long long>(static_cast<uint32_t>(row)) * p.group_mul) >> p.group_shift);
 }
@@ -81,24 +105,25 @@ __device__ __forceinline__ int row_limit(const PaParams& p, const Item& it, int 
 }
 
 // ---- the table of row tiles ----------------------------------------------------------------------------------
-__device__ __forceinline__ int block_exclusive(int v, int* scan, int* total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  int x = v;
+__device__ __forceinline__ int warp_inclusive(int x) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int y = __shfl_up_sync(0xffffffffu, x, o);
     if (lane >= o) x += y;
   }
+  return x;
+}
+__device__ __forceinline__ int block_exclusive(int v, int* scan, int* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int x = warp_inclusive(v);
   __syncthreads();  // `scan` may still be read
   if (lane == 31) scan[warp] = x;
   __syncthreads();
-  int before = 0, all = 0;
-  for (int i = 0; i < warps; ++i) {
-    before += i < warp ? scan[i] : 0;
-    all += scan[i];
-  }
-  *total = all;
-  return before + x - v;
+  const int y = warp_inclusive(lane < warps ? scan[lane] : 0);
+  *total = __shfl_sync(0xffffffffu, y, 31);
+  const int before = __shfl_sync(0xffffffffu, y, max(warp - 1, 0));
+  return (warp > 0 ? before : 0) + x - v;
 }
 __device__ __forceinline__ long long block_sum64(long long v, long long* scan) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
@@ -107,20 +132,18 @@ __device__ __forceinline__ long long block_sum64(long long v, long long* scan) {
   __syncthreads();
   if (lane == 0) scan[warp] = v;
   __syncthreads();
-  long long s = 0;
-  for (int i = 0; i < warps; ++i) s += scan[i];
-  return s;
-}
-__device__ __forceinline__ int block_max(int v, int* scan) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  v = lane < warps ? scan[lane] : 0;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ int block_max(int v, int* scan) {  // (of values that are not negative)
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  v = __reduce_max_sync(0xffffffffu, v);
   __syncthreads();
   if (lane == 0) scan[warp] = v;
   __syncthreads();
-  int m = scan[0];
-  for (int i = 1; i < warps; ++i) m = max(m, scan[i]);
-  return m;
+  return __reduce_max_sync(0xffffffffu, lane < warps ? scan[lane] : 0);
 }
 
 __device__ __forceinline__ void sequence(const PaParams& p, int i, int& q0, int& lq, int& k0, int& lk) {
@@ -316,6 +339,8 @@ __device__ __forceinline__ Item find_item(const PaParams& p, const PaTile* tile,
   const int end = static_cast<int>(static_cast<long long>(n_all) * (part + 1) / t.pieces);
   it.edge = row_limit(p, it, 0);
   it.keys = row_limit(p, it, it.rows - 1);
+  it.last[0] = it.dual ? it.keys : row_limit(p, it, 127);
+  it.last[1] = it.keys;
   if (it.dual) {
     const int mid = begin + (end - begin + 1) / 2;
     it.begin[0] = begin;
@@ -323,7 +348,7 @@ __device__ __forceinline__ Item find_item(const PaParams& p, const PaTile* tile,
     it.end[1] = end;
   } else {
     it.begin[0] = it.begin[1] = begin;
-    const int end0 = (row_limit(p, it, 127) + kPaKeys - 1) / kPaKeys;
+    const int end0 = (it.last[0] + kPaKeys - 1) / kPaKeys;
     it.end[0] = max(min(end, end0), begin);
     it.end[1] = end;
   }
@@ -339,29 +364,42 @@ __device__ __forceinline__ void ring_at(uint32_t pos, uint32_t& slot, uint32_t& 
   phase = lap & 1;
 }
 
-// Ring position of the value tile of step k of a stream, counted from the item's first slot (the order that the loads are in)
+// Ring positions of the key and value tiles of step k of a stream, counted from the item's first slot, in the order of the loads:
+// two tiles: K(0) | V(0) K(1) | V(1) K(2) ... for both streams; one tile: K0(0) K1(0) | V0(0) K0(1) V1(0) K1(1) | ...
 template <typename C>
-__device__ __forceinline__ uint32_t v_position(const Item& it, int s, int k, int n0, int n1) {
-  if (!it.dual) return C::kK * (k + 1) + C::kV * k;
+__device__ __forceinline__ uint32_t v_position(bool dual, int s, int k, int n0, int n1) {
+  if (!dual) return C::kK * (k + 1) + C::kV * k;
   if (s == 0) return C::kK * (k + 1 + min(k + 1, n1)) + C::kV * (k + min(k, n1));
   return C::kK * (min(k + 2, n0) + k + 1) + C::kV * (2 * k + 1);
 }
+template <typename C>
+__device__ __forceinline__ uint32_t k_position(bool dual, int s, int k, int n0, int n1) {
+  if (k == 0) return dual && s == 1 ? C::kK : 0;
+  return v_position<C>(dual, s, k - 1, n0, n1) + C::kV;
+}
+
+// Steps of a stream: whole tiles, but for the last one's where no row sees the rest
+template <typename C>
+__device__ __forceinline__ int item_steps(const Item& it, int s) {
+  const int begin = it.begin[s], n = it.end[s] - begin;
+  return max(0, min(n * C::kSteps, (it.last[s] - begin * kPaKeys + C::kStep - 1) / C::kStep));
+}
 
 // K and V tiles through the ring, and the items
-template <typename C, int DQK, int DV>
+template <typename C>
 __device__ __forceinline__ void role_load(const PaParams& p, const Ctx& x, const CUtensorMap* mk, const CUtensorMap* mv, PaHead* head,
                                           const PaTile* tile) {
   Ctl* c = x.c;
   const int lane = threadIdx.x & 31;
   const int tiles = head->tiles, pieces = head->pieces;
   uint32_t pos = 0;
-  bool ok = true;
   long long w = blockIdx.x;
-  for (uint32_t n_item = 0; ok; ++n_item) {
+  for (uint32_t n_item = 0;; ++n_item) {
     const uint32_t buf = n_item & 1;
-    ok = wait_warp(c->mempty[buf], ((n_item >> 1) & 1) ^ 1, p.status, 80);
-    if (!ok) break;
-    const Item it = find_item(p, tile, tiles, pieces, w);
+    wait_warp(c, c->mempty[buf], ((n_item >> 1) & 1) ^ 1, p.status, 80);
+    Item it = find_item(p, tile, tiles, pieces, w);
+    if (*reinterpret_cast<volatile int*>(&c->expired)) it.valid = 0;
+    it.valid = __shfl_sync(0xffffffffu, it.valid, 0);
     if (lane == 0) {
       c->item[buf] = it;
       mbar_arrive(smem_u32(&c->mfull[buf]));
@@ -369,43 +407,38 @@ __device__ __forceinline__ void role_load(const PaParams& p, const Ctx& x, const
     if (!it.valid) break;
     int next = 0;
     if (lane == 0 && !p.self_plan) next = atomicAdd(&head->next, 1);  // (its answer is due at the end of the item)
-    auto load = [&](int slots, int cols, const CUtensorMap* map, int key_tile, bool edge) {
-      for (int i = 0; i < slots && ok; ++i, ++pos) {
+    auto load = [&](int slots, const CUtensorMap* map, int key_tile, bool edge) {
+      for (int i = 0; i < slots; ++i, ++pos) {
         uint32_t slot, phase;
         ring_at<C::kRing>(pos, slot, phase);
-        ok = wait_warp(c->empty[slot], phase ^ 1, p.status, 81);
-        if (!ok) return;
-        if (elect_one()) {
+        wait_warp(c, c->empty[slot], phase ^ 1, p.status, 81);
+        if (elect_one() && !*reinterpret_cast<volatile int*>(&c->expired)) {
           const uint32_t bar = smem_u32(edge ? &c->raw[slot] : &c->full[slot]), dst = x.ring + slot * C::kSlot;
           mbar_arrive_expect_tx(bar, C::kSlot);
 #pragma unroll
           for (int bx = 0; bx < C::kSlotBoxes; ++bx) {
-            asm volatile(
-                "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
-                    dst + bx * kBox),
-                "l"(map), "r"((i * C::kSlotBoxes + bx) * 64), "r"(it.head), "r"(it.k0 + key_tile * kPaKeys), "r"(bar)
-                : "memory");
+            tma_load_3d(dst + bx * kBox, map, (i * C::kSlotBoxes + bx) * 64, it.head, it.k0 + key_tile * kPaKeys, bar);
           }
         }
         __syncwarp();
       }
     };
     const int n0 = it.end[0] - it.begin[0], n1 = it.end[1] - it.begin[1], n = max(n0, n1);
-    auto key = [&](int s, int k) { load(C::kK, DQK, mk, it.begin[s] + k, false); };
+    auto key = [&](int s, int k) { load(C::kK, mk, it.begin[s] + k, false); };
     auto value = [&](int s, int k) {
       const int j = it.begin[s] + k;
-      load(C::kV, DV, mv, j, (j + 1) * kPaKeys > it.edge);
+      load(C::kV, mv, j, (j + 1) * kPaKeys > it.edge);
     };
     if (!it.dual) {  // both streams read stream 1's tiles
       if (n > 0) key(1, 0);
-      for (int k = 0; k < n && ok; ++k) {
+      for (int k = 0; k < n; ++k) {
         value(1, k);
         if (k + 1 < n) key(1, k + 1);
       }
     } else {
       if (n0 > 0) key(0, 0);
       if (n1 > 0) key(1, 0);
-      for (int k = 0; k < n && ok; ++k) {
+      for (int k = 0; k < n; ++k) {
         if (k < n0) value(0, k);
         if (k + 1 < n0) key(0, k + 1);
         if (k < n1) value(1, k);
@@ -414,81 +447,112 @@ __device__ __forceinline__ void role_load(const PaParams& p, const Ctx& x, const
     }
     w = p.self_plan ? w + gridDim.x : static_cast<long long>(gridDim.x) + __shfl_sync(0xffffffffu, next, 0);
   }
-  // whoever gave up: copies in flight arrive before the CTA ends
-  if (!ok) {
-    for (uint32_t i = pos > C::kRing ? pos - C::kRing : 0; i < pos; ++i) {
-      uint32_t slot, phase;
-      ring_at<C::kRing>(i, slot, phase);
-      const long long t0 = clock64();
-      while (!mbar_test_wait(smem_u32(&c->full[slot]), phase) && clock64() - t0 < kWaitBudgetCycles / 16) {}
-    }
+  if (*reinterpret_cast<volatile int*>(&c->expired)) {  // copies in flight arrive before the CTA ends
+    const long long t0 = clock64();
+    while (clock64() - t0 < kWaitBudgetCycles / 64) {}
   }
 }
 
-// Queries of the item's tile into shared memory; value tiles at the edge: keys that no row sees become zeros (they may be another
+// a * 0 + b of pairs: not a number once a value was not finite
+template <bool F16>
+__device__ __forceinline__ uint32_t times_zero(uint32_t a, uint32_t b) {
+  uint32_t d;
+  if constexpr (F16) asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(0u), "r"(b));
+  else asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(0u), "r"(b));
+  return d;
+}
+
+// Queries of the item's tiles into shared memory; value tiles at the edge: keys that no row sees become zeros (they may be another
 // sequence's, or anything), and of keys that some rows do not see, values that are not finite become zeros (0 * inf is not 0); the
 // rows that do see them get them added at the end.
-template <typename C, int DQK, int DV, typename T>
-__device__ __forceinline__ void role_queries(const PaParams& p, const Ctx& x, int s) {
+template <typename C, int DQK, int DV, bool F16>
+__device__ __forceinline__ void role_queries(const PaParams& p, const Ctx& x, const CUtensorMap* mq) {
   Ctl* c = x.c;
   const int lane = threadIdx.x & 31;
-  uint32_t base = 0, edges = 0, raw_phase = 0;
-  bool ok = true;
-  for (uint32_t n_item = 0; ok; ++n_item) {
+  uint32_t base = 0, raw_phase = 0;
+  for (uint32_t n_item = 0;; ++n_item) {
     const uint32_t buf = n_item & 1;
-    ok = wait_warp(c->mfull[buf], (n_item >> 1) & 1, p.status, 82);
-    if (!ok) break;
-    const Item it = c->item[buf];
+    wait_warp(c, c->mfull[buf], (n_item >> 1) & 1, p.status, 82);
+    if (*reinterpret_cast<volatile int*>(&c->expired)) break;
+    const Item& it = c->item[buf];
     if (!it.valid) break;
-    if (lane == 0) c->odd[buf][s] = 0;
-    if (n_item > 0) ok = wait_warp(c->qempty, (n_item - 1) & 1, p.status, 83);
-    if (!ok) break;
-    if (s == 0 || !it.dual) {
-      const int piece = lane & 7;
-      const T* q = reinterpret_cast<const T*>(p.q) + piece * 8;
-#pragma unroll 4
-      for (int i = 0; i < 32; ++i) {
-        const int r = i * 4 + (lane >> 3), row = s * 128 + r;
-        const bool in = row < it.rows;
-        const int token = row_token(p, it.row0 + (in ? row : 0));
-        const int h = it.head * p.group + it.row0 + (in ? row : 0) - token * p.group;
-        const T* src = q + static_cast<int64_t>(it.q0 + token) * p.q_token + h * p.q_head;
-        const uint32_t dst = x.q + s * C::kQ + r * 128 + ((piece ^ (r & 7)) << 4);
+    const bool dual = it.dual;
+    if (lane == 0) c->odd[buf] = 0;
+    if (n_item > 0) wait_warp(c, c->qempty, (n_item - 1) & 1, p.status, 83);
+    if (*reinterpret_cast<volatile int*>(&c->expired)) break;
+    const int q0 = it.q0, row0 = it.row0, rows = it.rows, head = it.head * p.group;
+    if (p.q_map) {
+      // rows are token-major, so a tile is a box of 128 / group tokens x group heads; what lies behind the sequence is not written
+      if (elect_one()) {
+        const int token = q0 + row_token(p, row0);
 #pragma unroll
-        for (int ch = 0; ch < DQK / 64; ++ch) cp_async_16(dst + ch * kBox, src + ch * 64, in ? 16 : 0);
+        for (int s = 0; s < 2; ++s) {
+          const uint32_t bar = smem_u32(&c->qfull[s]);
+          if (s == 1 && dual) {
+            mbar_arrive(bar);
+          } else {
+            mbar_arrive_expect_tx(bar, C::kQ);
+#pragma unroll
+            for (int ch = 0; ch < DQK / 64; ++ch) {
+              tma_load_3d(x.q + s * C::kQ + ch * kBox, mq, ch * 64, head, token + (s == 1 ? row_token(p, 128) : 0), bar);
+            }
+          }
+        }
       }
-      asm volatile("cp.async.wait_all;" ::: "memory");
+      __syncwarp();
+    } else {
+      const int piece = lane & 7;
+      const uint16_t* q = reinterpret_cast<const uint16_t*>(p.q) + piece * 8;
+      for (int s = 0; s < 2; ++s) {
+        if (s == 0 || !dual) {
+#pragma unroll 4
+          for (int i = 0; i < 32; ++i) {
+            const int r = i * 4 + (lane >> 3), row = s * 128 + r;
+            const bool in = row < rows;
+            const int token = row_token(p, row0 + (in ? row : 0));
+            const int h = head + row0 + (in ? row : 0) - token * p.group;
+            const uint16_t* src = q + static_cast<int64_t>(q0 + token) * p.q_token + h * p.q_head;
+            const uint32_t dst = x.q + s * C::kQ + r * 128 + ((piece ^ (r & 7)) << 4);
+#pragma unroll
+            for (int ch = 0; ch < DQK / 64; ++ch) cp_async_16(dst + ch * kBox, src + ch * 64, in ? 16 : 0);
+          }
+          asm volatile("cp.async.wait_all;" ::: "memory");
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&c->qfull[s]));
+      }
     }
-    fence_proxy_async();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(smem_u32(&c->qfull[s]));
 
-    const int n0 = it.end[0] - it.begin[0], n1 = it.end[1] - it.begin[1], n = max(n0, n1);
-    const int first = it.edge / kPaKeys;  // tile
-    for (int k = max(0, min(first - it.begin[0], first - it.begin[1])); k < n && ok; ++k) {
-      for (int st = it.dual ? 0 : 1; st < 2 && ok; ++st) {
-        const int j = it.begin[st] + k;
+    const int b0 = it.begin[0], b1 = it.begin[1], n0 = it.end[0] - b0, n1 = it.end[1] - b1, n = max(n0, n1);
+    const int edge = it.edge, keys = it.keys, first = edge / kPaKeys;  // first tile at the edge
+    for (int k = max(0, min(first - b0, first - b1)); k < n; ++k) {
+      for (int st = dual ? 0 : 1; st < 2; ++st) {
+        const int j = (st == 0 ? b0 : b1) + k;
         if (k >= (st == 0 ? n0 : n1) || j < first) continue;
-        const uint32_t at = base + v_position<C>(it, st, k, n0, n1);
-        for (int i = 0; i < C::kV; ++i, ++edges) {
+        const uint32_t at = base + v_position<C>(dual, st, k, n0, n1);
+        for (int i = 0; i < C::kV; ++i) {
           uint32_t slot, phase;
           ring_at<C::kRing>(at + i, slot, phase);
-          const uint32_t rp = (raw_phase >> slot) & 1;
+          wait_warp(c, c->raw[slot], (raw_phase >> slot) & 1, p.status, 84);
           raw_phase ^= 1u << slot;
-          if ((edges & 1) != static_cast<uint32_t>(s)) continue;
-          ok = wait_warp(c->raw[slot], rp, p.status, 84);
-          if (!ok) break;
-          const int from = max(it.edge - j * kPaKeys, 0), keep = it.keys - j * kPaKeys;
-          bool odd = false;
-          for (int r = (from & ~3) + (lane >> 3); r < 128; r += 4) {
-            if (r < from) continue;
-#pragma unroll
-            for (int bx = 0; bx < C::kSlotBoxes; ++bx) {
-              const uint32_t a = x.ring + slot * C::kSlot + bx * kBox + r * 128 + (lane & 7) * 16;
-              if (r >= keep) {
-                sts_v4u(a, make_uint4(0, 0, 0, 0));
-              } else {
-                uint4 v = lds_v4u(a);
+          // rows [from, keep) are looked at, rows from keep on cleared; a lane has 16 bytes of every fourth row
+          const int from = max(edge - j * kPaKeys, 0), keep = min(max(keys - j * kPaKeys, 0), kPaKeys);
+          const uint32_t mine = x.ring + slot * C::kSlot + (lane >> 3) * 128 + (lane & 7) * 16;
+          const int r0 = lane >> 3;
+          for (int bx = 0; bx < C::kSlotBoxes; ++bx) {
+            const uint32_t a = mine + bx * kBox;
+            uint32_t seen = 0;
+#pragma unroll 8
+            for (int g = from >> 2; g < (keep + 3) >> 2; ++g) {
+              const uint4 v = lds_v4u(a + g * 512);
+              seen = times_zero<F16>(v.x, times_zero<F16>(v.y, times_zero<F16>(v.z, times_zero<F16>(v.w, seen))));
+            }
+            if ((seen & 0x7fff7fffu) != 0) {  // (rows below `from` or from keep on may have set it off)
+              for (int g = from >> 2; g < (keep + 3) >> 2; ++g) {
+                const int r = g * 4 + r0;
+                if (r < from || r >= keep) continue;
+                uint4 v = lds_v4u(a + g * 512);
                 uint32_t* u = reinterpret_cast<uint32_t*>(&v);
                 bool bad = false;
 #pragma unroll
@@ -504,151 +568,175 @@ __device__ __forceinline__ void role_queries(const PaParams& p, const Ctx& x, in
                   }
                 }
                 if (bad) {
-                  sts_v4u(a, v);
-                  odd = true;
+                  sts_v4u(a + g * 512, v);
+                  c->odd[buf] = 1;
                 }
               }
             }
+            for (int g = keep >> 2; g < kPaKeys / 4; ++g) {
+              if (g * 4 + r0 >= keep) sts_v4u(a + g * 512, make_uint4(0, 0, 0, 0));
+            }
           }
-          if (odd) c->odd[buf][s] = 1;
           fence_proxy_async();
           __syncwarp();
           if (lane == 0) mbar_arrive(smem_u32(&c->full[slot]));
         }
       }
     }
-    base += (it.dual ? n0 + n1 : n) * (C::kK + C::kV);
+    base += (dual ? n0 + n1 : n) * (C::kK + C::kV);
     if (lane == 0) mbar_arrive(smem_u32(&c->mempty[buf]));
   }
 }
 
-template <typename C, int DQK, int DV>
+// The MMAs of one stream: S(0) S(1) | PV(0) S(2) | PV(1) S(3) ... One thread does all of it: a converged warp that elects a lane for
+// every batch took twice as long from a barrier to the last product.
+template <typename C, int DQK, int DV, int S>
 __device__ __forceinline__ void role_mma(const PaParams& p, const Ctx& x) {
   Ctl* c = x.c;
-  const int lane = threadIdx.x & 31;
-  constexpr uint32_t kIdS = umma_idesc(kCFmtF32, C::kFmt, C::kFmt, 0, 0, 128, kPaKeys);
-  uint32_t pos = 0, np[2] = {0, 0};
-  bool ok = true;
-  auto score = [&](int s, int q_tile, uint32_t at, bool last_use) {
+  constexpr uint32_t kIdS = umma_idesc(kCFmtF32, C::kFmt, C::kFmt, 0, 0, 128, C::kStep);
+  constexpr uint32_t kIdO = umma_idesc(kCFmtF32, C::kFmt, C::kFmt, 0, 1, 128, DV), kIdO64 = umma_idesc(kCFmtF32, C::kFmt, C::kFmt, 0, 1, 128, 64);
+  const uint32_t t_o = x.tmem + C::kColO + S * DV;
+  const uint32_t sfull = smem_u32(&c->sfull[S][0]), pfree = smem_u32(&c->pfree[S]), empty = smem_u32(&c->empty[0]), full = smem_u32(&c->full[0]);
+  const uint32_t pfull = smem_u32(&c->pfull[S][0]);
+  const uint64_t k_desc = umma_desc_kmajor_sw128(x.ring), v_desc = desc_mnmajor_sw128(x.ring, kBox, 1024);
+  uint32_t base = 0, ns = 0, np = 0;
+  // A slot is free once both streams have read it; one that only this stream reads is given back twice. Before its next load is
+  // waited for, the one before, maybe of the other stream alone, must have been given back: a barrier tells even laps from odd ones.
+  auto loaded = [&](uint32_t at) {
+    const uint32_t lap = at / C::kRing, slot = at - lap * C::kRing;
+    if (lap > 0) wait_bar(c, empty + slot * 8, (lap - 1) & 1, p.status, 86);
+    wait_bar(c, full + slot * 8, lap & 1, p.status, 87);
+  };
+  auto give_back = [&](uint32_t slot, bool alone) {
+    tc_commit(empty + slot * 8);
+    if (alone) tc_commit(empty + slot * 8);
+  };
+  for (uint32_t n_item = 0;; ++n_item) {
+    const uint32_t buf = n_item & 1;
+    wait_bar(c, smem_u32(&c->mfull[buf]), (n_item >> 1) & 1, p.status, 89);
+    if (*reinterpret_cast<volatile int*>(&c->expired)) break;
+    const Item& it = c->item[buf];
+    if (!it.valid) break;
+    const bool dual = it.dual;
+    const int n0 = it.end[0] - it.begin[0], n1 = it.end[1] - it.begin[1], n = item_steps<C>(it, S);
+    const int q_tile = dual ? 0 : S;
     const uint64_t a = umma_desc_kmajor_sw128(x.q + q_tile * C::kQ);
+    // (its own barrier as well, so that it is never more than a phase behind)
+    wait_bar(c, smem_u32(&c->qfull[S]), n_item & 1, p.status, 90);
+    if (q_tile != S) wait_bar(c, smem_u32(&c->qfull[q_tile]), n_item & 1, p.status, 90);
+    auto score = [&](int i) {
+      const int k = i / C::kSteps, h = i % C::kSteps;
+      const bool last = h == C::kSteps - 1 || i + 1 == n, alone = dual || (S == 1 && k >= n0);
+      const uint32_t at = base + k_position<C>(dual, S, k, n0, n1), t_s = x.tmem + S * 128 + (ns & 1) * 64;
 #pragma unroll
-    for (int i = 0; i < C::kK; ++i) {
-      uint32_t slot, phase;
-      ring_at<C::kRing>(at + i, slot, phase);
-      if (!wait_warp(c->full[slot], phase, p.status, 85)) return false;
-      tc_fence_after();
-      if (elect_one()) {
-        const uint64_t b = umma_desc_kmajor_sw128(x.ring + slot * C::kSlot);
+      for (int j = 0; j < C::kK; ++j) {
+        if (h == 0) loaded(at + j);
+        const uint32_t slot = (at + j) % C::kRing;
+        const uint64_t b = k_desc + (slot * (C::kSlot >> 4) + h * (C::kStep * 128 >> 4));
+        tc_fence_after();
 #pragma unroll
         for (int bx = 0; bx < C::kSlotBoxes; ++bx) {
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) {
-            mma_f16_ss(x.tmem + s * 128, a + ((i * C::kSlotBoxes + bx) * (kBox >> 4) + kk * 2), b + (bx * (kBox >> 4) + kk * 2), kIdS,
-                       (i | bx | kk) != 0);
+            mma_f16_ss(t_s, a + ((j * C::kSlotBoxes + bx) * (kBox >> 4) + kk * 2), b + (bx * (kBox >> 4) + kk * 2), kIdS, (j | bx | kk) != 0);
           }
         }
-        if (last_use) tc_commit(smem_u32(&c->empty[slot]));
-        if (i == C::kK - 1) tc_commit(smem_u32(&c->sfull[s]));
+        if (j == C::kK - 1) tc_commit(sfull + (ns & 1) * 8);
+        if (last) give_back(slot, alone);
       }
-      __syncwarp();
-    }
-    return true;
-  };
-  auto value = [&](int s, uint32_t at, bool first, bool last, bool last_use) {
-    if (!wait_warp(c->pfull[s], np[s] & 1, p.status, 86)) return false;
-    ++np[s];
-    const uint32_t d = x.tmem + 256 + s * 128, a = x.tmem + s * 128;
-    uint32_t slot[C::kV], phase;
-#pragma unroll
-    for (int i = 0; i < C::kV; ++i) {
-      ring_at<C::kRing>(at + i, slot[i], phase);
-      if (!wait_warp(c->full[slot[i]], phase, p.status, 87)) return false;
-    }
-    tc_fence_after();
-    if (elect_one()) {
-      // boxes of 64 value columns side by side: one product of dv columns, unless the ring wraps between them
-      const bool joined = C::kV == 1 || slot[C::kV - 1] == slot[0] + C::kV - 1;
-      if (joined) {
-        constexpr uint32_t id = umma_idesc(kCFmtF32, C::kFmt, C::kFmt, 0, 1, 128, DV);
-        const uint64_t b = desc_mnmajor_sw128(x.ring + slot[0] * C::kSlot, kBox, 1024);
-#pragma unroll
-        for (int kk = 0; kk < kPaKeys / 16; ++kk) mma_f16_ts(d, a + kk * 8, b + kk * 128, id, !first || kk > 0);
-      } else {
-        constexpr uint32_t id = umma_idesc(kCFmtF32, C::kFmt, C::kFmt, 0, 1, 128, 64);
-#pragma unroll
-        for (int i = 0; i < C::kV; ++i) {
-          const uint64_t b = desc_mnmajor_sw128(x.ring + slot[i] * C::kSlot, kBox, 1024);
-#pragma unroll
-          for (int kk = 0; kk < kPaKeys / 16; ++kk) mma_f16_ts(d + i * 64, a + kk * 8, b + kk * 128, id, !first || kk > 0);
-        }
-      }
-      if (last_use) {
-#pragma unroll
-        for (int i = 0; i < C::kV; ++i) tc_commit(smem_u32(&c->empty[slot[i]]));
-      }
-      if (last) tc_commit(smem_u32(&c->ofull[s]));
-    }
-    __syncwarp();
-    return true;
-  };
-  for (uint32_t n_item = 0; ok; ++n_item) {
-    const uint32_t buf = n_item & 1;
-    ok = wait_warp(c->mfull[buf], (n_item >> 1) & 1, p.status, 88);
-    if (!ok) break;
-    const Item it = c->item[buf];
-    if (!it.valid) break;
-    const bool dual = it.dual;
-    const int n0 = it.end[0] - it.begin[0], n1 = it.end[1] - it.begin[1], n = max(n0, n1);
-    uint32_t k_next = 0, v_now = 0;
-    // slots in the order of the loads; in an item of two tiles stream 1 reads what stream 0 has read, and frees it
-    auto take = [&](int slots) {
-      const uint32_t at = pos;
-      pos += slots;
-      return at;
+      ++ns;
+      if (i + 1 == n) tc_commit(smem_u32(&c->qempty));  // the queries have been read
     };
-    ok = wait_warp(c->qfull[0], n_item & 1, p.status, 89) && wait_warp(c->qfull[1], n_item & 1, p.status, 90);
-    if (ok && n0 > 0) {
-      k_next = take(C::kK);
-      ok = score(0, 0, k_next, dual);
-    }
-    if (ok && n1 > 0) ok = score(1, dual ? 0 : 1, !dual && n0 > 0 ? k_next : take(C::kK), true);
-    if (ok && n <= 1 && elect_one()) tc_commit(smem_u32(&c->qempty));
-    __syncwarp();
-    for (int k = 0; k < n && ok; ++k) {
-      if (k < n0) {
-        v_now = take(C::kV);
-        ok = value(0, v_now, k == 0, k + 1 == n0, dual);
-        if (ok && k + 1 < n0) {
-          k_next = take(C::kK);
-          ok = score(0, 0, k_next, dual);
+    if (n == 0) tc_commit(smem_u32(&c->qempty));
+    for (int i = 0; i < 2 && i < n; ++i) score(i);
+    for (int i = 0; i < n; ++i, ++np) {
+      const int k = i / C::kSteps, h = i % C::kSteps;
+      const uint32_t at = base + v_position<C>(dual, S, k, n0, n1), t_p = x.tmem + S * 128 + (np & 1) * 64;
+      uint32_t slot[C::kV];
+#pragma unroll
+      for (int j = 0; j < C::kV; ++j) {
+        slot[j] = (at + j) % C::kRing;
+        if (h == 0) loaded(at + j);
+      }
+      wait_bar(c, pfull + (np & 1) * 8, (np >> 1) & 1, p.status, 88);
+      tc_fence_after();
+      // boxes of 64 value columns side by side: one product of dv columns, unless the ring wraps between them
+      if (C::kV == 1 || slot[C::kV - 1] == slot[0] + C::kV - 1) {
+        const uint64_t b = v_desc + (slot[0] * (C::kSlot >> 4) + h * (C::kStep * 128 >> 4));
+#pragma unroll
+        for (int kk = 0; kk < C::kStep / 16; ++kk) mma_f16_ts(t_o, t_p + kk * 8, b + kk * 128, kIdO, i > 0 || kk > 0);
+      } else {
+#pragma unroll
+        for (int j = 0; j < C::kV; ++j) {
+          const uint64_t b = v_desc + (slot[j] * (C::kSlot >> 4) + h * (C::kStep * 128 >> 4));
+#pragma unroll
+          for (int kk = 0; kk < C::kStep / 16; ++kk) mma_f16_ts(t_o + j * 64, t_p + kk * 8, b + kk * 128, kIdO64, i > 0 || kk > 0);
         }
       }
-      if (ok && k < n1) {
-        ok = value(1, !dual && k < n0 ? v_now : take(C::kV), k == 0, k + 1 == n1, true);
-        if (ok && k + 1 < n1) ok = score(1, dual ? 0 : 1, !dual && k + 1 < n0 ? k_next : take(C::kK), true);
+      tc_commit(pfree);
+      if (i + 1 == n) tc_commit(smem_u32(&c->ofull[S]));
+      if (h == C::kSteps - 1 || i + 1 == n) {
+#pragma unroll
+        for (int j = 0; j < C::kV; ++j) give_back(slot[j], dual || (S == 1 && k >= n0));
       }
-      // the queries have been read once the last scores are there
-      if (ok && k + 2 == n && elect_one()) tc_commit(smem_u32(&c->qempty));
-      __syncwarp();
+      if (i + 2 < n) score(i + 2);
     }
-    if (lane == 0) mbar_arrive(smem_u32(&c->mempty[buf]));
+    base += (dual ? n0 + n1 : max(n0, n1)) * (C::kK + C::kV);
+    mbar_arrive(smem_u32(&c->mempty[buf]));
   }
   // what was issued completes before the CTA ends
-  if (elect_one()) tc_commit(smem_u32(&c->drain));
-  __syncwarp();
-  wait_warp(c->drain, 0, p.status, 91);
+  tc_commit(smem_u32(&c->drain[S]));
+  wait_bar(c, smem_u32(&c->drain[S]), 0, p.status, 91);
 }
 
-__device__ __forceinline__ void fma2(float& x, float& y, float a, float b) {  // (x, y) = (x, y) * a + b
-  asm("{\n\t.reg .b64 v, s, t;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 s, {%2, %2};\n\tmov.b64 t, {%3, %3};\n\t"
-      "fma.rn.f32x2 v, v, s, t;\n\tmov.b64 {%0, %1}, v;\n\t}"
-      : "+f"(x), "+f"(y)
-      : "f"(a), "f"(b));
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 u, v, w;\n\tmov.b64 u, {%2, %3};\n\tmov.b64 v, {%4, %5};\n\tmov.b64 w, {%6, %7};\n\t"
+      "fma.rn.f32x2 u, u, v, w;\n\tmov.b64 {%0, %1}, u;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
 }
-__device__ __forceinline__ void add2(float& x, float& y, float a, float b) {
-  asm("{\n\t.reg .b64 v, s;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 s, {%2, %3};\n\tadd.rn.f32x2 v, v, s;\n\tmov.b64 {%0, %1}, v;\n\t}"
-      : "+f"(x), "+f"(y)
-      : "f"(a), "f"(b));
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 u, v;\n\tmov.b64 u, {%2, %3};\n\tmov.b64 v, {%4, %5};\n\tadd.rn.f32x2 u, u, v;\n\tmov.b64 {%0, %1}, u;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+// largest of three; a NaN stays one
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// 2^x of a pair on the FMA pipe: x = n + f, |f| <= 1/2, n from the sum with 1.5 * 2^23; 2^f by the polynomial of degree four with
+// p(0) = 1 and the smallest relative error on that interval (2.8e-6; computed by Lawson's iteration); n goes to the exponent. 0 for
+// x <= -127. The exponential unit gives 16 values a clock and SM, half of what the products of a tile take: a share of
+// the exponentials goes this way.
+template <int N, int M>
+__device__ __forceinline__ void exp2_fma(float2 (&x)[M]) {  // of the first N pairs
+  float2 t[N > 0 ? N : 1], y[N > 0 ? N : 1];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    x[i] = make_float2(fmaxf(x[i].x, -127.f), fmaxf(x[i].y, -127.f));
+    t[i] = add2(x[i], both(12582912.f));
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = add2(x[i], fma2(t[i], both(-1.f), both(12582912.f)));
+#pragma unroll
+  for (int i = 0; i < N; ++i) y[i] = fma2(x[i], both(0x1.3a02ccp-7f), both(0x1.c9fc46p-5f));
+#pragma unroll
+  for (int i = 0; i < N; ++i) y[i] = fma2(x[i], y[i], both(0x1.ec0378p-3f));
+#pragma unroll
+  for (int i = 0; i < N; ++i) y[i] = fma2(x[i], y[i], both(0x1.62e12cp-1f));
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    y[i] = fma2(x[i], y[i], both(1.f));
+    x[i].x = __int_as_float(__float_as_int(y[i].x) + (__float_as_int(t[i].x) << 23));
+    x[i].y = __int_as_float(__float_as_int(y[i].y) + (__float_as_int(t[i].y) << 23));
+  }
 }
 template <bool F16>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
@@ -670,56 +758,61 @@ __device__ __forceinline__ void role_softmax(const PaParams& p, const Ctx& x, in
   Ctl* c = x.c;
   const int lane = threadIdx.x & 31, r = threadIdx.x & 127;
   const uint32_t lanes = static_cast<uint32_t>((threadIdx.x >> 5) & 3) << 21;
-  const uint32_t t_s = x.tmem + lanes + s * 128, t_o = x.tmem + lanes + 256 + s * 128;
+  const uint32_t t_o = x.tmem + lanes + C::kColO + s * DV;
   const float sl = p.scale_log2;
-  uint32_t ns = 0, no[2] = {0, 0}, nx = 0;
-  bool ok = true;
-  for (uint32_t n_item = 0; ok; ++n_item) {
+  uint32_t ns = 0, no = 0, nx = 0;
+  const uint32_t sfull = smem_u32(&c->sfull[s][0]), pfull = smem_u32(&c->pfull[s][0]);
+  for (uint32_t n_item = 0;; ++n_item) {
     const uint32_t buf = n_item & 1;
-    ok = wait_warp(c->mfull[buf], (n_item >> 1) & 1, p.status, 92);
-    if (!ok) break;
+    wait_warp(c, c->mfull[buf], (n_item >> 1) & 1, p.status, 92);
+    if (*reinterpret_cast<volatile int*>(&c->expired)) break;
     const Item& it = c->item[buf];
     if (!it.valid) break;
-    const int begin = it.begin[s], n = it.end[s] - begin, n1 = it.end[1] - it.begin[1];
+    const int n = item_steps<C>(it, s), key0 = it.begin[s] * kPaKeys;
     const int row = (it.dual ? 0 : s * 128) + r;
     const bool mine = row < it.rows;
     const int limit = row_limit(p, it, mine ? row : it.rows - 1);
     const int sure = row_limit(p, it, it.dual ? 0 : s * 128);  // keys that all rows of the stream see
     float m = -INFINITY, l = 0.f;                              // maximum (of the scores as they are) and sum
     for (int k = 0; k < n; ++k, ++ns) {
-      ok = wait_warp(c->sfull[s], ns & 1, p.status, 93);
-      if (!ok) break;
+      const uint32_t t_s = x.tmem + lanes + s * 128 + (ns & 1) * 64;
+      wait_bar(c, sfull + (ns & 1) * 8, (ns >> 1) & 1, p.status, 93);
+      __syncwarp();
       tc_fence_after();
-      uint32_t u[4][32];
+      uint32_t u[C::kStep / 32][32];
+      float(&v)[C::kStep / 32][32] = reinterpret_cast<float(&)[C::kStep / 32][32]>(u);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) tmem_ld_32x32b_x32(t_s + i * 32, u[i]);
+      for (int h = 0; h < C::kStep / 32; ++h) tmem_ld_32x32b_x32(t_s + 32 * h, u[h]);
       tc_wait_ld();
-      float(&v)[4][32] = reinterpret_cast<float(&)[4][32]>(u);
-      const int j = begin + k;
-      if ((j + 1) * kPaKeys > sure) {
-        const int left = limit - j * kPaKeys;
+      const int left = limit - (key0 + k * C::kStep);
+      if (key0 + (k + 1) * C::kStep > sure) {
 #pragma unroll
-        for (int i = 0; i < 128; ++i) v[i >> 5][i & 31] = i < left ? v[i >> 5][i & 31] : -INFINITY;
+        for (int i = 0; i < C::kStep; ++i) v[i >> 5][i & 31] = i < left ? v[i >> 5][i & 31] : -INFINITY;
       }
-      float top[4];
+      float top[C::kStep / 16];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        top[i] = v[i][0];
+      for (int h = 0; h < C::kStep / 16; ++h) {
+        const float* w = &v[h >> 1][(h & 1) * 16];
+        top[h] = max3(w[0], w[1], w[2]);
 #pragma unroll
-        for (int e = 1; e < 32; ++e) top[i] = fmaxf(top[i], v[i][e]);
+        for (int e = 3; e < 15; e += 2) top[h] = max3(top[h], w[e], w[e + 1]);
+        top[h] = max3(top[h], w[15], h > 0 ? top[h - 1] : w[15]);
       }
-      const float t = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      float t = top[C::kStep / 16 - 1];
+      if (t == INFINITY) t = NAN;  // inf - inf: what the row comes to in any case
       if (k == 0) {
         m = t;
       } else {
-        // the first tile's maximum mostly stays good enough: the output is rescaled when it is more than 2^8 behind
-        const bool raise = (t - m) * sl > kLag || (m == -INFINITY && t > m);
+        // the first maximum mostly stays good enough: the output is rescaled when it is more than 2^8 behind
+        const bool raise = m == -INFINITY ? t != m : !((t - m) * sl <= kLag);
         if (__any_sync(0xffffffffu, raise)) {
           const float f = raise ? (m == -INFINITY ? 0.f : ex2f((m - t) * sl)) : 1.f;
           m = raise ? t : m;
           l *= f;
-          // (the scores of this tile are complete, so the value product before them is)
-#pragma unroll
+          // the value product before (the one before that came ahead of these scores)
+          wait_warp(c, c->pfree[s], (ns - 1) & 1, p.status, 94);
+          tc_fence_after();
+#pragma unroll 1
           for (int i = 0; i < DV / 32; ++i) {
             uint32_t o[32];
             tmem_ld_32x32b_x32(t_o + i * 32, o);
@@ -730,48 +823,49 @@ __device__ __forceinline__ void role_softmax(const PaParams& p, const Ctx& x, in
           }
         }
       }
-      const float shift = C::kBias - (m == -INFINITY ? 0.f : m * sl);
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      const float2 shift = both(C::kBias - (m == -INFINITY ? 0.f : m * sl));
+      float2 sum[2] = {both(0.f), both(0.f)};
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t w[32];
+      for (int h = 0; h < C::kStep / 32; ++h) {
+        uint32_t w[16];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          float& a = v[2 * h + (e >> 4)][(2 * e) & 31];
-          float& b = v[2 * h + (e >> 4)][(2 * e + 1) & 31];
-          fma2(a, b, sl, shift);
-          a = ex2f(a);
-          b = ex2f(b);
-          add2(sum[2 * (e & 1)], sum[2 * (e & 1) + 1], a, b);
-          w[e] = pack16<F16>(a, b);
+        for (int g = 0; g < 16; g += 8) {
+          float2 y[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = fma2(make_float2(v[h][2 * (g + e)], v[h][2 * (g + e) + 1]), both(sl), shift);
+          exp2_fma<kFmaPairs>(y);
+#pragma unroll
+          for (int e = kFmaPairs; e < 8; ++e) y[e] = make_float2(ex2f(y[e].x), ex2f(y[e].y));
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            sum[e & 1] = add2(sum[e & 1], y[e]);
+            w[g + e] = pack16<F16>(y[e].x, y[e].y);
+          }
         }
-        tmem_st_32x32b_x32(t_s + h * 32, w);
+        tmem_st_32x32b_x16(t_s + h * 16, w);
       }
-      l += (sum[0] + sum[2]) + (sum[1] + sum[3]);
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&c->pfull[s]));
+      if (lane == 0) mbar_arrive(pfull + (ns & 1) * 8);
+      l += (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
     }
-    if (!ok) break;
 
     // ---- the item's output
-    const int n_other = n1;
-    if (s == 0 && !it.dual && n1 > 0) ++no[1];  // (another stream's phase that is not waited for here)
     if (n > 0) {
-      ok = wait_warp(c->ofull[s], no[s] & 1, p.status, 94);
-      ++no[s];
-      if (!ok) break;
+      wait_warp(c, c->ofull[s], no & 1, p.status, 96);
+      ++no;
+      tc_fence_after();
     }
     const float e = m * sl;  // exponent of the maximum
     if (it.dual && s == 1) {
-      ok = wait_warp(c->xempty, (nx & 1) ^ 1, p.status, 95);
-      if (!ok) break;
+      wait_warp(c, c->xempty, (nx & 1) ^ 1, p.status, 97);
       c->xch[r] = make_float2(n > 0 ? e : -INFINITY, l);
+      tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&c->xfull));
       // stream 0 reads this stream's output: the next item's first probabilities come after that
-      ok = wait_warp(c->xempty, nx & 1, p.status, 96);
+      wait_warp(c, c->xempty, nx & 1, p.status, 97);
       ++nx;
       if (lane == 0) mbar_arrive(smem_u32(&c->mempty[buf]));
       continue;
@@ -779,15 +873,10 @@ __device__ __forceinline__ void role_softmax(const PaParams& p, const Ctx& x, in
     float f0 = 1.f, f1 = 0.f, top = n > 0 ? e : -INFINITY, all = l;
     bool two = false;
     if (it.dual) {
-      ok = wait_warp(c->xfull, nx & 1, p.status, 97);
+      wait_warp(c, c->xfull, nx & 1, p.status, 98);
       ++nx;
-      if (ok && n_other > 0) {
-        ok = wait_warp(c->ofull[1], no[1] & 1, p.status, 98);
-        ++no[1];
-      }
-      if (!ok) break;
       const float2 o = c->xch[r];
-      two = n_other > 0;
+      two = it.end[1] > it.begin[1];
       if (two) {
         const float best = fmaxf(top, o.x);
         f0 = top == -INFINITY ? 0.f : ex2f(top - best);
@@ -797,7 +886,7 @@ __device__ __forceinline__ void role_softmax(const PaParams& p, const Ctx& x, in
       }
     }
     tc_fence_after();
-    const bool odd = (c->odd[buf][0] | c->odd[buf][1]) != 0;
+    const bool odd = c->odd[buf] != 0;
     const int token = it.q0 + row_token(p, it.row0 + row);
     const int h = it.head * p.group + (it.row0 + row) - row_token(p, it.row0 + row) * p.group;
     const float inv = it.slot >= 0 ? 1.f : (all == 0.f ? 0.f : 1.f / all);
@@ -817,7 +906,7 @@ __device__ __forceinline__ void role_softmax(const PaParams& p, const Ctx& x, in
         for (int q = 0; q < 32; ++q) y[q] = 0.f;
       }
       if (two) {
-        tmem_ld_32x32b_x32(t_o + 128 + i * 32, a);
+        tmem_ld_32x32b_x32(t_o + DV + i * 32, a);
         tc_wait_ld();
 #pragma unroll
         for (int q = 0; q < 32; ++q) y[q] = fmaf(__uint_as_float(a[q]), f1, y[q]);
@@ -867,9 +956,9 @@ __device__ __forceinline__ void role_softmax(const PaParams& p, const Ctx& x, in
 
 template <int DQK, int DV, bool F16>
 __global__ void __launch_bounds__(kThreads, 1)
-pa_kernel(const PaParams p, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
+pa_kernel(const PaParams p, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+          const __grid_constant__ CUtensorMap map_v) {
   using C = Cfg<DQK, DV, F16>;
-  using T = uint16_t;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t at = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* base = smem_raw + (at - smem_u32(smem_raw));
@@ -879,26 +968,30 @@ pa_kernel(const PaParams p, const __grid_constant__ CUtensorMap map_k, const __g
     for (int i = 0; i < C::kRing; ++i) {
       mbar_init(smem_u32(&c->full[i]), 1);
       mbar_init(smem_u32(&c->raw[i]), 1);
-      mbar_init(smem_u32(&c->empty[i]), 1);
+      mbar_init(smem_u32(&c->empty[i]), 2);  // both streams
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&c->qfull[i]), 1);
-      mbar_init(smem_u32(&c->sfull[i]), 1);
-      mbar_init(smem_u32(&c->pfull[i]), 4);
+      for (int j = 0; j < 2; ++j) {
+        mbar_init(smem_u32(&c->sfull[i][j]), 1);
+        mbar_init(smem_u32(&c->pfull[i][j]), 4);
+      }
+      mbar_init(smem_u32(&c->pfree[i]), 1);
       mbar_init(smem_u32(&c->ofull[i]), 1);
       mbar_init(smem_u32(&c->mfull[i]), 1);
-      mbar_init(smem_u32(&c->mempty[i]), 11);  // warps 0, 2, 3 and the softmax's eight
+      mbar_init(smem_u32(&c->mempty[i]), 11);  // warps 0, 1, 3 and the softmax's eight
+      mbar_init(smem_u32(&c->drain[i]), 1);
     }
-    mbar_init(smem_u32(&c->qempty), 1);
+    mbar_init(smem_u32(&c->qempty), 2);
     mbar_init(smem_u32(&c->xfull), 4);
     mbar_init(smem_u32(&c->xempty), 4);
-    mbar_init(smem_u32(&c->drain), 1);
+    c->expired = 0;
     fence_mbar_init();
   }
   if (warp == 0) {
     tmem_alloc(smem_u32(&c->tmem), kTmemCols);
     tmem_relinquish();
-  } else if (warp == 1 && p.tk > 0 && elect_one()) {
+  } else if (warp == 2 && p.tk > 0 && elect_one()) {
     tma_prefetch_desc(&map_k);
     tma_prefetch_desc(&map_v);
   }
@@ -919,9 +1012,14 @@ pa_kernel(const PaParams p, const __grid_constant__ CUtensorMap map_k, const __g
   const Ctx x{c, at, at + 2 * C::kQ, c->tmem};
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    if (warp == 0) role_mma<C, DQK, DV>(p, x);
-    else if (warp == 1) role_load<C, DQK, DV>(p, x, &map_k, &map_v, head, tile);
-    else role_queries<C, DQK, DV, T>(p, x, warp - 2);
+    if (warp < 2) {
+      if (elect_one()) {
+        if (warp == 0) role_mma<C, DQK, DV, 0>(p, x);
+        else role_mma<C, DQK, DV, 1>(p, x);
+      }
+      __syncwarp();
+    } else if (warp == 2) role_load<C>(p, x, &map_k, &map_v, head, tile);
+    else role_queries<C, DQK, DV, F16>(p, x, &map_q);
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     role_softmax<C, DV, F16>(p, x, warp < 8 ? 0 : 1);
@@ -991,17 +1089,17 @@ __global__ void __launch_bounds__(256) pa_merge_kernel(const PaParams p) {
 }
 
 template <int DQK, int DV, bool F16>
-cudaError_t launch(const PaParams& p, const void* tmap_k, const void* tmap_v, int ctas, cudaStream_t stream) {
+cudaError_t launch(const PaParams& p, const void* tmap_q, const void* tmap_k, const void* tmap_v, int ctas, cudaStream_t stream) {
   cudaError_t e = cudaFuncSetAttribute(pa_kernel<DQK, DV, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) return e;
   if (!p.self_plan) {
-    pa_plan_kernel<<<1, 1024, 0, stream>>>(p, ctas);
+    pa_plan_kernel<<<1, p.max_tiles <= kPaSmallTiles ? kPaSmallTiles : 1024, 0, stream>>>(p, ctas);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     count_launch();
   }
   e = launch_maybe_pdl(pa_kernel<DQK, DV, F16>, dim3(ctas), dim3(kThreads), kSmem, stream, !p.self_plan, p,
-                       *reinterpret_cast<const CUtensorMap*>(tmap_k), *reinterpret_cast<const CUtensorMap*>(tmap_v));
+                       *reinterpret_cast<const CUtensorMap*>(tmap_q), *reinterpret_cast<const CUtensorMap*>(tmap_k), *reinterpret_cast<const CUtensorMap*>(tmap_v));
   if (e != cudaSuccess) return e;
   count_launch();
   if (p.slots > 0) {
@@ -1013,12 +1111,18 @@ cudaError_t launch(const PaParams& p, const void* tmap_k, const void* tmap_v, in
 
 }  // namespace
 
-cudaError_t launch_prompt_attention(const PaParams& p, int dqk, int dv, int dtype, const void* tmap_k, const void* tmap_v, int ctas,
-                                    cudaStream_t stream) {
+cudaError_t launch_prompt_attention(const PaParams& p, int dqk, int dv, int dtype, const void* tmap_q, const void* tmap_k,
+                                    const void* tmap_v, int ctas, cudaStream_t stream) {
   const bool f16 = dtype == PTO_DT_F16;
-  if (dqk == 64 && dv == 64) return f16 ? launch<64, 64, true>(p, tmap_k, tmap_v, ctas, stream) : launch<64, 64, false>(p, tmap_k, tmap_v, ctas, stream);
-  if (dqk == 128 && dv == 128) return f16 ? launch<128, 128, true>(p, tmap_k, tmap_v, ctas, stream) : launch<128, 128, false>(p, tmap_k, tmap_v, ctas, stream);
-  if (dqk == 192 && dv == 128) return f16 ? launch<192, 128, true>(p, tmap_k, tmap_v, ctas, stream) : launch<192, 128, false>(p, tmap_k, tmap_v, ctas, stream);
+#define PA_LAUNCH(a, b)                                                          \
+  if (dqk == a && dv == b) {                                                     \
+    return f16 ? launch<a, b, true>(p, tmap_q, tmap_k, tmap_v, ctas, stream)     \
+               : launch<a, b, false>(p, tmap_q, tmap_k, tmap_v, ctas, stream);   \
+  }
+  PA_LAUNCH(64, 64)
+  PA_LAUNCH(128, 128)
+  PA_LAUNCH(192, 128)
+#undef PA_LAUNCH
   return cudaErrorInvalidValue;
 }
 

@@ -33,6 +33,7 @@ struct PaParams {
   int tq, tk, b, hq, hkv, group;
   uint32_t group_mul;  // row / group = row * group_mul >> group_shift
   int group_shift;
+  int q_map;  // query tiles are boxes of a tensor map (the group divides 128)
   int causal, head_set;  // head_set: key heads that are worked on together (what L2 holds)
   float scale, scale_log2;
   int max_tiles, slot_rows;
@@ -45,7 +46,7 @@ struct PaParams {
   int32_t* status;
 };
 
-cudaError_t launch_prompt_attention(const PaParams& p, int dqk, int dv, int dtype, const void* tmap_k, const void* tmap_v, int ctas,
-                                    cudaStream_t stream);
+cudaError_t launch_prompt_attention(const PaParams& p, int dqk, int dv, int dtype, const void* tmap_q, const void* tmap_k,
+                                    const void* tmap_v, int ctas, cudaStream_t stream);
 
 }  // namespace pto
