@@ -1412,6 +1412,7 @@ int pto_prompt_attention(const void* query, const void* key, const void* value, 
     rc = make_heads_map(&map_q, query, tq, hq, dqk, strides[0], strides[1], group);
     if (rc != PTO_OK) return rc;
   }
+  p.out_wide = (reinterpret_cast<uintptr_t>(attention_out) & 31u) == 0 && strides[6] % 16 == 0 && strides[7] % 16 == 0;
   uint8_t* base = reinterpret_cast<uint8_t*>(workspace);
   p.q = query;
   p.out = attention_out;

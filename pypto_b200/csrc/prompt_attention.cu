@@ -16,6 +16,8 @@
 #include "prompt_attention.cuh"
 #include "sfa_common.cuh"
 
+#include <climits>
+
 namespace pto {
 namespace {
 
@@ -38,10 +40,10 @@ struct Cfg {
   // f16 probabilities are kept away from its subnormal values: times 2^4 (a maximum that lags by 2^8 leaves them below 2^12)
   static constexpr float kBias = F16 ? 4.f : 0.f;
 };
-constexpr int kFmaPairs = 0;  // of eight pairs of probabilities, those whose exponentials the FMA pipe computes
+constexpr int kFmaPairs = 1;  // of eight pairs of probabilities, those whose exponentials the FMA pipe computes
 constexpr float kLag = 8.f;  // a maximum is raised, and the output rescaled, once it is 2^8 behind
 
-struct Item {
+struct alignas(16) Item {
   int valid, dual;
   int q0, row0, rows;        // first token of the sequence, first row, rows of the item
   int k0, lk, seen;          // first key, keys; row r sees min(lk, seen + token) keys
@@ -54,7 +56,7 @@ struct Item {
 constexpr int kMaxRing = 12;
 struct Ctl {
   unsigned long long full[kMaxRing], raw[kMaxRing], empty[kMaxRing];
-  unsigned long long qfull[2], qempty, sfull[2][2], pfull[2][2], pfree[2], ofull[2], xfull, xempty, mfull[2], mempty[2], drain[2];
+  unsigned long long qfull[2], qempty[2], sfull[2][2], pfull[2][2], pfree[2], ofull[2], xfull, xempty, mfull[2], mempty[2], drain[2];
   Item item[2];
   int odd[2];  // values that are not finite were taken out of an item's tiles
   uint32_t tmem;
@@ -163,14 +165,16 @@ constexpr int kBuckets = 256;
 struct PlanScratch {
   long long sum[32];
   int scan[32];
-  int n[kPaSmallTiles];  // small tables: key tiles of a row tile; others: places of the buckets
+  int n[kPaSmallTiles];          // small tables: key tiles of a row tile; others: places of the buckets
+  int first[kPaSmallTiles + 1];  // small tables: first row tile of a sequence
 };
 static_assert(kBuckets <= kPaSmallTiles, "buckets");
 
 // Row tiles, longest first, and how many pieces each is cut into. Called by all threads of a block. `head`, `tile`, `first`: the
 // table. `ctas`: CTAs that will work.
 __device__ void build_table(const PaParams& p, PaHead* head, PaTile* tile, int* first, PlanScratch* s, int ctas) {
-  const int nt = blockDim.x, tid = threadIdx.x;
+  const int nt = blockDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = nt >> 5;
+  if (p.max_tiles <= kPaSmallTiles) first = s->first;  // (b is at most max_tiles)
   int total = 0;
   for (int base = 0; base < p.b; base += nt) {
     const int i = base + tid;
@@ -211,6 +215,7 @@ __device__ void build_table(const PaParams& p, PaHead* head, PaTile* tile, int* 
     if (tid < total) {
       mine = look(tid);
       sum = longest = n = tile_keys(p, mine);
+      s->n[tid] = n;
     }
   } else {
     for (int t = tid; t < total; t += nt) {
@@ -222,25 +227,36 @@ __device__ void build_table(const PaParams& p, PaHead* head, PaTile* tile, int* 
   sum = block_sum64(sum, s->sum) * p.hkv;
   longest = block_max(longest, s->scan);
 
-  // Pieces of at most `piece` key tiles. Fewer items than CTAs: the shortest pieces that are no more than CTAs. More: a CTA's share
-  // in four, so that the last ones to finish are not far apart (the partial results of a piece cost about a tile's time).
+  // Pieces of at most `piece` key tiles. Where that evens out, no more pieces than CTAs: the shortest ones of which there are no more.
+  // Otherwise a third of a CTA's share each, so that the last ones to finish are not far apart (a piece costs a CTA about two tiles'
+  // time beside its keys; 16 sequences of 1 to 16384 keys x 8 heads in one wave: 117 us, in thirds PA_T16).
   int piece = max(longest, 1);
   if (p.slots > 0 && longest > kPaMinPiece) {
+    const int share = static_cast<int>((sum + ctas - 1) / ctas);
+    const int third = max((share + 2) / 3, kPaMinPiece);
     if (static_cast<long long>(total) * p.hkv <= ctas && small) {
-      int lo = kPaMinPiece, hi = longest;
+      // each warp counts for a length of its own
+      int lo = kPaMinPiece, hi = longest;  // (as long as the longest: one piece each, which fits)
       while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        const long long all = block_sum64((n + mid - 1) / mid + (tid < total && n == 0), s->sum);
-        if (all * p.hkv <= ctas) hi = mid;
-        else lo = mid + 1;
+        const int mid = lo + (hi - lo) * warp / warps;
+        int all = 0;
+        for (int t = lane; t < total; t += 32) all += max((s->n[t] + mid - 1) / mid, 1);
+        all = __reduce_add_sync(0xffffffffu, all);
+        __syncthreads();
+        if (lane == 0) s->scan[warp] = all * p.hkv <= ctas ? mid : INT_MAX;
+        __syncthreads();
+        // the shortest that fits, and the longest below it that does not
+        const int fits = static_cast<int>(__reduce_min_sync(0xffffffffu, static_cast<unsigned>(lane < warps ? s->scan[lane] : INT_MAX)));
+        const int mine_mid = lo + (hi - lo) * lane / warps;
+        const int fails = static_cast<int>(__reduce_max_sync(0xffffffffu, lane < warps && s->scan[min(lane, warps - 1)] == INT_MAX ? mine_mid : 0));
+        hi = min(hi, fits);
+        lo = max(lo, min(fails + 1, hi));
       }
-      piece = lo;
-    } else {
-      const long long share = (sum + 4 * ctas - 1) / (4 * ctas);
-      if (longest > 2 * share) piece = static_cast<int>(max(share, static_cast<long long>(kPaMinPiece)));
+      piece = lo <= share + share / 4 + 1 ? lo : third;
+    } else if (longest > 2 * third) {
+      piece = third;
     }
   }
-
   if (piece < longest) {  // (the workspace is counted so that they fit)
     const int k = (n + piece - 1) / piece;
     const long long slots = small ? block_sum64(k > 1 ? k : 0, s->sum) * p.hkv : 2 * sum / piece;
@@ -249,8 +265,6 @@ __device__ void build_table(const PaParams& p, PaHead* head, PaTile* tile, int* 
 
   int pieces_all = 0, slots_all = 0;
   if (small) {
-    if (tid < total) s->n[tid] = n;
-    __syncthreads();
     if (tid < total) {
       int rank = 0;
       for (int t = 0; t < total; ++t) rank += s->n[t] > n || (s->n[t] == n && t < tid);
@@ -313,18 +327,27 @@ __device__ __forceinline__ Item find_item(const PaParams& p, const PaTile* tile,
   const int heads = min(p.head_set, p.hkv - set * p.head_set);
   const int which = rem / heads;
   it.head = set * p.head_set + rem - which * heads;
-  // the last tile whose first piece is at most `which`: 32 probes a step
+  // the last tile whose first piece is at most `which`: 32 probes a step, whole in the last one
   const int lane = threadIdx.x & 31;
   int lo = 0, n = tiles;
-  while (n > 1) {
+  while (n > 32) {
     const int step = (n + 31) / 32;
-    const int probe = lo + lane * step;
-    const unsigned below = __ballot_sync(0xffffffffu, lane * step < n && tile[probe].piece <= which);
+    const unsigned below = __ballot_sync(0xffffffffu, lane * step < n && tile[lo + lane * step].piece <= which);
     const int last = 31 - __clz(below);  // (lane 0's holds always)
     lo += last * step;
     n = min(step, n - last * step);
   }
-  const PaTile t = tile[lo];
+  PaTile t = {};
+  if (lane < n) t = tile[lo + lane];
+  const int at = 31 - __clz(__ballot_sync(0xffffffffu, lane < n && t.piece <= which));
+  t.q0 = __shfl_sync(0xffffffffu, t.q0, at);
+  t.lq = __shfl_sync(0xffffffffu, t.lq, at);
+  t.k0 = __shfl_sync(0xffffffffu, t.k0, at);
+  t.lk = __shfl_sync(0xffffffffu, t.lk, at);
+  t.row0 = __shfl_sync(0xffffffffu, t.row0, at);
+  t.pieces = __shfl_sync(0xffffffffu, t.pieces, at);
+  t.piece = __shfl_sync(0xffffffffu, t.piece, at);
+  t.slot = __shfl_sync(0xffffffffu, t.slot, at);
   const int part = which - t.piece;
   it.valid = 1;
   it.q0 = t.q0;
@@ -381,8 +404,8 @@ __device__ __forceinline__ uint32_t k_position(bool dual, int s, int k, int n0, 
 // Steps of a stream: whole tiles, but for the last one's where no row sees the rest
 template <typename C>
 __device__ __forceinline__ int item_steps(const Item& it, int s) {
-  const int begin = it.begin[s], n = it.end[s] - begin;
-  return max(0, min(n * C::kSteps, (it.last[s] - begin * kPaKeys + C::kStep - 1) / C::kStep));
+  const int begin = s == 0 ? it.begin[0] : it.begin[1], n = (s == 0 ? it.end[0] : it.end[1]) - begin;
+  return max(0, min(n * C::kSteps, ((s == 0 ? it.last[0] : it.last[1]) - begin * kPaKeys + C::kStep - 1) / C::kStep));
 }
 
 // K and V tiles through the ring, and the items
@@ -478,15 +501,13 @@ __device__ __forceinline__ void role_queries(const PaParams& p, const Ctx& x, co
     if (!it.valid) break;
     const bool dual = it.dual;
     if (lane == 0) c->odd[buf] = 0;
-    if (n_item > 0) wait_warp(c, c->qempty, (n_item - 1) & 1, p.status, 83);
-    if (*reinterpret_cast<volatile int*>(&c->expired)) break;
     const int q0 = it.q0, row0 = it.row0, rows = it.rows, head = it.head * p.group;
     if (p.q_map) {
       // rows are token-major, so a tile is a box of 128 / group tokens x group heads; what lies behind the sequence is not written
-      if (elect_one()) {
-        const int token = q0 + row_token(p, row0);
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
+      const int token = q0 + row_token(p, row0);
+      for (int s = 0; s < 2; ++s) {
+        if (n_item > 0) wait_warp(c, c->qempty[s], (n_item - 1) & 1, p.status, 83);
+        if (elect_one() && !*reinterpret_cast<volatile int*>(&c->expired)) {
           const uint32_t bar = smem_u32(&c->qfull[s]);
           if (s == 1 && dual) {
             mbar_arrive(bar);
@@ -498,12 +519,13 @@ __device__ __forceinline__ void role_queries(const PaParams& p, const Ctx& x, co
             }
           }
         }
+        __syncwarp();
       }
-      __syncwarp();
     } else {
       const int piece = lane & 7;
       const uint16_t* q = reinterpret_cast<const uint16_t*>(p.q) + piece * 8;
       for (int s = 0; s < 2; ++s) {
+        if (n_item > 0) wait_warp(c, c->qempty[s], (n_item - 1) & 1, p.status, 83);
         if (s == 0 || !dual) {
 #pragma unroll 4
           for (int i = 0; i < 32; ++i) {
@@ -615,7 +637,7 @@ __device__ __forceinline__ void role_mma(const PaParams& p, const Ctx& x) {
     const uint32_t buf = n_item & 1;
     wait_bar(c, smem_u32(&c->mfull[buf]), (n_item >> 1) & 1, p.status, 89);
     if (*reinterpret_cast<volatile int*>(&c->expired)) break;
-    const Item& it = c->item[buf];
+    const Item it = c->item[buf];  // (in registers: under the products' reads a look into shared memory takes some 200 cycles)
     if (!it.valid) break;
     const bool dual = it.dual;
     const int n0 = it.end[0] - it.begin[0], n1 = it.end[1] - it.begin[1], n = item_steps<C>(it, S);
@@ -624,6 +646,7 @@ __device__ __forceinline__ void role_mma(const PaParams& p, const Ctx& x) {
     // (its own barrier as well, so that it is never more than a phase behind)
     wait_bar(c, smem_u32(&c->qfull[S]), n_item & 1, p.status, 90);
     if (q_tile != S) wait_bar(c, smem_u32(&c->qfull[q_tile]), n_item & 1, p.status, 90);
+    auto queries_read = [&]() { tc_commit(smem_u32(&c->qempty[q_tile])); };
     auto score = [&](int i) {
       const int k = i / C::kSteps, h = i % C::kSteps;
       const bool last = h == C::kSteps - 1 || i + 1 == n, alone = dual || (S == 1 && k >= n0);
@@ -645,9 +668,10 @@ __device__ __forceinline__ void role_mma(const PaParams& p, const Ctx& x) {
         if (last) give_back(slot, alone);
       }
       ++ns;
-      if (i + 1 == n) tc_commit(smem_u32(&c->qempty));  // the queries have been read
+      if (i + 1 == n) queries_read();
     };
-    if (n == 0) tc_commit(smem_u32(&c->qempty));
+    if (n == 0) queries_read();
+    if (S == 1) mbar_arrive(smem_u32(&c->qempty[dual ? 1 : 0]));  // the tile that it does not read
     for (int i = 0; i < 2 && i < n; ++i) score(i);
     for (int i = 0; i < n; ++i, ++np) {
       const int k = i / C::kSteps, h = i % C::kSteps;
@@ -753,6 +777,18 @@ __device__ __forceinline__ float to_float(uint16_t v) {
   else return __uint_as_float(static_cast<uint32_t>(v) << 16);
 }
 
+// 32 bytes of a row: one store where they lie on a 32-byte boundary
+__device__ __forceinline__ void store32(void* dst, const uint32_t (&w)[8], bool wide) {
+  if (wide) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                 "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+  } else {
+    reinterpret_cast<uint4*>(dst)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    reinterpret_cast<uint4*>(dst)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+}
+
 template <typename C, int DV, bool F16>
 __device__ __forceinline__ void role_softmax(const PaParams& p, const Ctx& x, int s) {
   Ctl* c = x.c;
@@ -766,9 +802,9 @@ __device__ __forceinline__ void role_softmax(const PaParams& p, const Ctx& x, in
     const uint32_t buf = n_item & 1;
     wait_warp(c, c->mfull[buf], (n_item >> 1) & 1, p.status, 92);
     if (*reinterpret_cast<volatile int*>(&c->expired)) break;
-    const Item& it = c->item[buf];
+    const Item it = c->item[buf];
     if (!it.valid) break;
-    const int n = item_steps<C>(it, s), key0 = it.begin[s] * kPaKeys;
+    const int n = item_steps<C>(it, s), key0 = (s == 0 ? it.begin[0] : it.begin[1]) * kPaKeys;
     const int row = (it.dual ? 0 : s * 128) + r;
     const bool mine = row < it.rows;
     const int limit = row_limit(p, it, mine ? row : it.rows - 1);
@@ -892,8 +928,11 @@ __device__ __forceinline__ void role_softmax(const PaParams& p, const Ctx& x, in
     const float inv = it.slot >= 0 ? 1.f : (all == 0.f ? 0.f : 1.f / all);
     f0 *= inv;
     f1 *= inv;
-#pragma unroll
-    for (int i = 0; i < DV / 32; ++i) {
+    uint8_t* dst = it.slot >= 0 ? reinterpret_cast<uint8_t*>(p.part_o + (static_cast<int64_t>(it.slot) * p.slot_rows + row) * DV)
+                                : reinterpret_cast<uint8_t*>(reinterpret_cast<uint16_t*>(p.out) + token * p.out_token + h * p.out_head);
+    const bool any = __any_sync(0xffffffffu, mine);
+#pragma unroll 1  // (code that runs once an item is kept small: it is fetched anew every time)
+    for (int i = 0; any && i < DV / 32; ++i) {
       uint32_t a[32];
       float y[32];
       if (n > 0) {
@@ -925,15 +964,20 @@ __device__ __forceinline__ void role_softmax(const PaParams& p, const Ctx& x, in
       }
       if (mine) {
         if (it.slot >= 0) {
-          float* dst = p.part_o + (static_cast<int64_t>(it.slot) * p.slot_rows + row) * DV + i * 32;
 #pragma unroll
-          for (int q = 0; q < 32; q += 4) *reinterpret_cast<float4*>(dst + q) = make_float4(y[q], y[q + 1], y[q + 2], y[q + 3]);
+          for (int q = 0; q < 4; ++q) {
+            uint32_t w[8];
+#pragma unroll
+            for (int e2 = 0; e2 < 8; ++e2) w[e2] = __float_as_uint(y[8 * q + e2]);
+            store32(dst + i * 128 + q * 32, w, true);
+          }
         } else {
-          uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + token * p.out_token + h * p.out_head + i * 32;
 #pragma unroll
-          for (int q = 0; q < 32; q += 8) {
-            *reinterpret_cast<uint4*>(dst + q) = make_uint4(pack16<F16>(y[q], y[q + 1]), pack16<F16>(y[q + 2], y[q + 3]),
-                                                            pack16<F16>(y[q + 4], y[q + 5]), pack16<F16>(y[q + 6], y[q + 7]));
+          for (int q = 0; q < 2; ++q) {
+            uint32_t w[8];
+#pragma unroll
+            for (int e2 = 0; e2 < 8; ++e2) w[e2] = pack16<F16>(y[16 * q + 2 * e2], y[16 * q + 2 * e2 + 1]);
+            store32(dst + i * 64 + q * 32, w, p.out_wide);
           }
         }
       }
@@ -982,7 +1026,8 @@ pa_kernel(const PaParams p, const __grid_constant__ CUtensorMap map_q, const __g
       mbar_init(smem_u32(&c->mempty[i]), 11);  // warps 0, 1, 3 and the softmax's eight
       mbar_init(smem_u32(&c->drain[i]), 1);
     }
-    mbar_init(smem_u32(&c->qempty), 2);
+    mbar_init(smem_u32(&c->qempty[0]), 2);
+    mbar_init(smem_u32(&c->qempty[1]), 1);
     mbar_init(smem_u32(&c->xfull), 4);
     mbar_init(smem_u32(&c->xempty), 4);
     c->expired = 0;

@@ -33,6 +33,7 @@ struct PaParams {
   int tq, tk, b, hq, hkv, group;
   uint32_t group_mul;  // row / group = row * group_mul >> group_shift
   int group_shift;
+  int out_wide;  // rows of the output on 32-byte boundaries
   int q_map;  // query tiles are boxes of a tensor map (the group divides 128)
   int causal, head_set;  // head_set: key heads that are worked on together (what L2 holds)
   float scale, scale_log2;
