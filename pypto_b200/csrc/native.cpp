@@ -38,7 +38,7 @@ constexpr auto kF32 = at::kFloat;
 // The tensors of one call: all contiguous, all on one CUDA device.
 class Call {
  public:
-  const at::Tensor* take(PyObject* o) {
+  const at::Tensor* take(PyObject* o, bool contiguous = true) {
     if (!ok_) return nullptr;
     const at::Tensor* t = nullptr;
     if (THPVariable_CheckExact(o)) {
@@ -52,10 +52,23 @@ class Call {
       if (THPVariable_CheckExact(inner)) t = &THPVariable_Unpack(inner);
       Py_DECREF(inner);
     }
-    if (t == nullptr || !t->is_cuda() || !t->is_contiguous()) return refuse();
+    if (t == nullptr || !t->is_cuda() || (contiguous && !t->is_contiguous())) return refuse();
     const int d = t->device().index();
     if (dev_ < 0) dev_ = d;
     if (d != dev_) return refuse();
+    return t;
+  }
+  // rows of 16-bit values of `dims` dims, last dim contiguous, every row on a 16-byte boundary
+  const at::Tensor* rows(PyObject* o, int64_t dims) {
+    const at::Tensor* t = take(o, /*contiguous=*/false);
+    if (t == nullptr) return nullptr;
+    if (t->dim() != dims || t->numel() == 0 || (t->scalar_type() != kBf16 && t->scalar_type() != kF16) || t->stride(dims - 1) != 1 ||
+        (reinterpret_cast<uintptr_t>(t->data_ptr()) & 15u) != 0) {
+      return refuse();
+    }
+    for (int64_t i = 0; i + 1 < dims; ++i) {
+      if (t->size(i) > 1 && t->stride(i) % 8 != 0) return refuse();
+    }
     return t;
   }
   // a tensor of a dtype and element count
@@ -121,9 +134,11 @@ template <typename F>
 PyObject* launch(const Call& c, size_t bytes, F&& f) {
   at::Tensor ws;  // (let go with the lock held, after the last use)
   cudaStream_t stream = nullptr;
-  if (!c.ok() || c.device() < 0 || !find_workspace(c, bytes, &ws, &stream)) Py_RETURN_FALSE;
-  void* const base = ws.data_ptr();
-  const size_t have = static_cast<size_t>(ws.numel());
+  if (!c.ok() || c.device() < 0) Py_RETURN_FALSE;
+  if (bytes == 0) stream = c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(c.device())).stream();  // (none needed)
+  else if (!find_workspace(c, bytes, &ws, &stream)) Py_RETURN_FALSE;
+  void* const base = bytes == 0 ? nullptr : ws.data_ptr();
+  const size_t have = bytes == 0 ? 0 : static_cast<size_t>(ws.numel());
   int rc = 0;
   {
     const WithoutLock without_lock;
@@ -493,6 +508,211 @@ PyObject* prolog(PyObject*, PyObject* const* a, Py_ssize_t n) {
   PTO_GUARD_END
 }
 
+// ---- operators around a prompt -------------------------------------------------------------------------
+
+int64_t stride_of(const at::Tensor* t, int64_t i) { return t->size(i) > 1 ? t->stride(i) : 0; }
+int row_dtype(const at::Tensor* t) { return t->scalar_type() == kBf16 ? PTO_DT_BF16 : PTO_DT_F16; }
+
+// query, key or None, positions, turns, query_out, key_out or None, query_weight or None, key_weight or None, eps, layout, rope_last,
+// rotary_dim, amplitude
+PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  PTO_GUARD_BEGIN
+  int64_t layout = 0, last = 0, rotary = 0;
+  double eps = 0, amplitude = 0;
+  if (n != 13 || !as_float(a[8], &eps) || !as_int(a[9], &layout) || !as_int(a[10], &last) || !as_int(a[11], &rotary) ||
+      !as_float(a[12], &amplitude) || eps < 0) {
+    Py_RETURN_FALSE;
+  }
+  Call c;
+  const at::Tensor *q = c.rows(a[0], 3), *qo = c.rows(a[4], 3);
+  if (!c.ok()) Py_RETURN_FALSE;
+  const at::Tensor *k = q, *ko = qo;
+  const bool with_key = a[1] != Py_None;
+  c.need(with_key == (a[5] != Py_None) && q->sizes() == qo->sizes() && qo->scalar_type() == q->scalar_type());
+  if (with_key) {
+    k = c.rows(a[1], 3);
+    ko = c.rows(a[5], 3);
+    if (!c.ok()) Py_RETURN_FALSE;
+    c.need(k->sizes() == ko->sizes() && k->size(0) == q->size(0) && k->scalar_type() == q->scalar_type() &&
+           ko->scalar_type() == q->scalar_type());
+  }
+  if (!c.ok()) Py_RETURN_FALSE;
+  const int64_t t = q->size(0);
+  const at::Tensor* pos = c.take(a[2]);
+  if (!c.ok()) Py_RETURN_FALSE;
+  c.need((pos->scalar_type() == kI32 || pos->scalar_type() == kI64) && pos->dim() == 1 && pos->size(0) == t && t <= INT32_MAX);
+  const void* turns = c.flat(a[3], kI64, rotary / 2);
+  const void *wq = nullptr, *wk = nullptr;
+  if (c.ok() && a[6] != Py_None) wq = c.flat(a[6], q->scalar_type(), q->size(2));
+  if (c.ok() && a[7] != Py_None) {
+    c.need(with_key);
+    wk = c.flat(a[7], k->scalar_type(), k->size(2));
+  }
+  if (!c.ok()) Py_RETURN_FALSE;
+  int64_t strides[8];
+  const at::Tensor* of[4] = {q, k, qo, ko};
+  for (int i = 0; i < 8; ++i) strides[i] = stride_of(of[i / 2], i % 2);
+  void *qp = q->data_ptr(), *kp = k->data_ptr(), *pp = pos->data_ptr(), *qop = qo->data_ptr(), *kop = ko->data_ptr();
+  const int dt = row_dtype(q), p64 = pos->scalar_type() == kI64, hq = static_cast<int>(q->size(1)), dq = static_cast<int>(q->size(2)),
+            hk = with_key ? static_cast<int>(k->size(1)) : 0, dk = static_cast<int>(k->size(2));
+  return launch(c, 0, [&](void*, size_t, pto_stream_t s) {
+    return pto_qk_norm_rope(qp, kp, pp, p64, static_cast<const uint64_t*>(turns), wq, wk, qop, kop, dt, static_cast<int>(t), hq, dq, hk, dk,
+                            strides, static_cast<int>(rotary), static_cast<int>(layout), static_cast<int>(last),
+                            static_cast<float>(amplitude), static_cast<float>(eps), s);
+  });
+  PTO_GUARD_END
+}
+
+// The caches of a write or a read: key_nope_2d, key_rope_2d, k_nope_scales, packed_kv_cache, each a tensor or None
+struct Caches {
+  void *nope, *rope, *scales, *packed;
+  int scale_dtype;
+  int64_t rows;
+};
+void take_caches(Call& c, PyObject* nope, PyObject* rope, PyObject* scales, PyObject* packed, int64_t width, bool with_rope, Caches& x) {
+  x = {nullptr, nullptr, nullptr, nullptr, PTO_DT_F32, 0};
+  c.need(width >= 128 && width % 128 == 0 && (nope != Py_None || packed != Py_None));
+  if (!c.ok()) return;
+  if (nope != Py_None) {
+    const at::Tensor *kn = c.take(nope), *sc = c.take(scales);
+    if (!c.ok()) return;
+    c.need(kn->scalar_type() == kI8 && kn->numel() > 0 && kn->numel() % width == 0 && with_rope == (rope != Py_None));
+    x.rows = kn->numel() / width;
+    c.need((sc->scalar_type() == kF32 || sc->scalar_type() == kF16) && sc->numel() == x.rows * (width / 128));
+    if (!c.ok()) return;
+    x.nope = kn->data_ptr();
+    x.scales = sc->data_ptr();
+    x.scale_dtype = sc->scalar_type() == kF32 ? PTO_DT_F32 : PTO_DT_F16;
+    if (with_rope) x.rope = c.flat(rope, kBf16, x.rows * 64);
+  } else {
+    c.need(rope == Py_None && scales == Py_None);
+  }
+  if (c.ok() && packed != Py_None) {
+    const at::Tensor* pk = c.take(packed);
+    if (!c.ok()) return;
+    c.need(width == 512 && pk->scalar_type() == kI8 && pk->numel() > 0 && pk->numel() % 656 == 0 &&
+           (x.nope == nullptr || pk->numel() == x.rows * 656));
+    x.rows = pk->numel() / 656;
+    x.packed = pk->data_ptr();
+  }
+}
+
+// key_nope, key_rope or None, cache_index, key_nope_2d, key_rope_2d, k_nope_scales, packed_kv_cache
+PyObject* kv_cache_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  PTO_GUARD_BEGIN
+  if (n != 7) Py_RETURN_FALSE;
+  Call c;
+  const at::Tensor* x = c.rows(a[0], 2);
+  if (!c.ok()) Py_RETURN_FALSE;
+  const int64_t t = x->size(0), width = x->size(1);
+  const at::Tensor* xr = nullptr;
+  if (a[1] != Py_None) {
+    xr = c.rows(a[1], 2);
+    if (!c.ok()) Py_RETURN_FALSE;
+    c.need(x->scalar_type() == kBf16 && xr->scalar_type() == kBf16 && xr->size(0) == t && xr->size(1) == 64);
+  }
+  c.need(a[6] == Py_None || xr != nullptr);
+  const void* ci = c.flat(a[2], kI64, t);
+  Caches k{};
+  take_caches(c, a[3], a[4], a[5], a[6], width, xr != nullptr, k);
+  c.need(t <= INT32_MAX && width <= INT32_MAX);
+  if (!c.ok()) Py_RETURN_FALSE;
+  void *xp = x->data_ptr(), *xrp = xr != nullptr ? xr->data_ptr() : nullptr;
+  const int64_t ld = stride_of(x, 0), ldr = xr != nullptr ? stride_of(xr, 0) : 0;
+  const int dt = row_dtype(x);
+  return launch(c, 256, [&](void* ws, size_t have, pto_stream_t s) {
+    return pto_kv_cache_write(xp, ld, xrp, ldr, static_cast<const int64_t*>(ci), dt, static_cast<int>(t), static_cast<int>(width),
+                              static_cast<int8_t*>(k.nope), k.rope, k.scales, k.scale_dtype, static_cast<int8_t*>(k.packed), k.rows, ws,
+                              have, s);
+  });
+  PTO_GUARD_END
+}
+
+// key_nope_2d, key_rope_2d, k_nope_scales, block_table, cu_seqlens, key_nope_out, key_rope_out or None, block_size, first or None,
+// packed_kv_cache
+PyObject* kv_cache_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  PTO_GUARD_BEGIN
+  int64_t bs = 0;
+  if (n != 10 || !as_int(a[7], &bs) || bs < 1 || (a[0] == Py_None) == (a[9] == Py_None)) Py_RETURN_FALSE;
+  Call c;
+  const at::Tensor* out = c.rows(a[5], 2);
+  if (!c.ok()) Py_RETURN_FALSE;
+  const int64_t rows = out->size(0), width = out->size(1);
+  const at::Tensor* ro = nullptr;
+  if (a[6] != Py_None) {
+    ro = c.rows(a[6], 2);
+    if (!c.ok()) Py_RETURN_FALSE;
+    c.need(out->scalar_type() == kBf16 && ro->scalar_type() == kBf16 && ro->size(0) == rows && ro->size(1) == 64);
+  }
+  c.need(a[9] == Py_None || out->scalar_type() == kBf16);
+  Caches k{};
+  take_caches(c, a[0], a[1], a[2], a[9], width, a[1] != Py_None, k);
+  c.need(ro == nullptr || k.packed != nullptr || k.rope != nullptr);
+  const at::Tensor *bt = c.take(a[3]), *cu = c.take(a[4]);
+  if (!c.ok()) Py_RETURN_FALSE;
+  c.need(cu->scalar_type() == kI32 && cu->dim() == 1 && cu->size(0) >= 2 && bt->scalar_type() == kI32 && bt->dim() == 2);
+  if (!c.ok()) Py_RETURN_FALSE;
+  const int64_t b = cu->size(0) - 1;
+  c.need(bt->size(0) == b && b <= INT32_MAX && bt->size(1) <= INT32_MAX && width <= INT32_MAX);
+  const void* first = nullptr;
+  if (c.ok() && a[8] != Py_None) {
+    const at::Tensor* f = c.take(a[8]);
+    if (!c.ok()) Py_RETURN_FALSE;
+    c.need(f->scalar_type() == kI32 && f->dim() == 1 && f->size(0) == b);
+    first = f->data_ptr();
+  }
+  if (!c.ok()) Py_RETURN_FALSE;
+  void *op = out->data_ptr(), *rop = ro != nullptr ? ro->data_ptr() : nullptr, *btp = bt->data_ptr(), *cup = cu->data_ptr();
+  const int64_t ld = stride_of(out, 0), ldr = ro != nullptr ? stride_of(ro, 0) : 0;
+  const int dt = row_dtype(out), mb = static_cast<int>(bt->size(1));
+  return launch(c, 256, [&](void* ws, size_t have, pto_stream_t s) {
+    return pto_kv_cache_read(static_cast<const int8_t*>(k.nope), k.rope, k.scales, k.scale_dtype, static_cast<const int8_t*>(k.packed), k.rows,
+                             static_cast<const int32_t*>(btp), static_cast<const int32_t*>(cup), static_cast<const int32_t*>(first),
+                             static_cast<int>(b), mb, static_cast<int>(bs), rows, static_cast<int>(width), op, ld, rop, ldr, dt, ws, have, s);
+  });
+  PTO_GUARD_END
+}
+
+// query, key, value, cu_seqlens_q, cu_seqlens_k, attention_out, softmax_scale, causal, lse_out or None
+PyObject* prompt_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  PTO_GUARD_BEGIN
+  double scale = 0;
+  int64_t causal = 0;
+  if (n != 9 || !as_float(a[6], &scale) || !as_int(a[7], &causal) || !(scale > 0.0 && scale <= 1e30)) Py_RETURN_FALSE;
+  Call c;
+  const at::Tensor *q = c.rows(a[0], 3), *k = c.rows(a[1], 3), *v = c.rows(a[2], 3), *out = c.rows(a[5], 3);
+  if (!c.ok()) Py_RETURN_FALSE;
+  const int64_t tq = q->size(0), hq = q->size(1), dqk = q->size(2), tk = v->size(0), hkv = v->size(1), dv = v->size(2);
+  c.need(k->size(0) == tk && k->size(1) == hkv && k->size(2) == dqk && out->size(0) == tq && out->size(1) == hq && out->size(2) == dv);
+  c.need(k->scalar_type() == q->scalar_type() && v->scalar_type() == q->scalar_type() && out->scalar_type() == q->scalar_type());
+  c.need(hq % hkv == 0 && tq <= INT32_MAX && tk <= INT32_MAX && hq <= INT32_MAX);
+  const at::Tensor *cq = c.take(a[3]), *ck = c.take(a[4]);
+  if (!c.ok()) Py_RETURN_FALSE;
+  c.need(cq->scalar_type() == kI32 && ck->scalar_type() == kI32 && cq->dim() == 1 && cq->size(0) >= 2 && ck->sizes() == cq->sizes());
+  void* lse = nullptr;
+  if (c.ok() && a[8] != Py_None) {
+    const at::Tensor* t = c.take(a[8]);
+    if (!c.ok()) Py_RETURN_FALSE;
+    c.need(t->scalar_type() == kF32 && t->dim() == 2 && t->size(0) == hq && t->size(1) == tq);
+    lse = t->data_ptr();
+  }
+  if (!c.ok()) Py_RETURN_FALSE;
+  const int b = static_cast<int>(cq->size(0) - 1), itq = static_cast<int>(tq), itk = static_cast<int>(tk), ihq = static_cast<int>(hq),
+            ihkv = static_cast<int>(hkv), idqk = static_cast<int>(dqk), idv = static_cast<int>(dv);
+  int64_t strides[8];
+  const at::Tensor* of[4] = {q, k, v, out};
+  for (int i = 0; i < 8; ++i) strides[i] = stride_of(of[i / 2], i % 2);
+  void *qp = q->data_ptr(), *kp = k->data_ptr(), *vp = v->data_ptr(), *op = out->data_ptr(), *cqp = cq->data_ptr(), *ckp = ck->data_ptr();
+  const int dt = row_dtype(q);
+  const size_t bytes = pto_prompt_attention_workspace_bytes(itq, itk, b, ihq, ihkv, idv);
+  if (bytes == 0) Py_RETURN_FALSE;
+  return launch(c, bytes, [&](void* ws, size_t have, pto_stream_t s) {
+    return pto_prompt_attention(qp, kp, vp, static_cast<const int32_t*>(cqp), static_cast<const int32_t*>(ckp), op, static_cast<float*>(lse), dt,
+                                itq, itk, b, ihq, ihkv, idqk, idv, strides, static_cast<float>(scale), static_cast<int>(causal), ws, have, s);
+  });
+  PTO_GUARD_END
+}
+
 // handle type (compat.Tensor), workspace dict, _lib.check
 PyObject* setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 3 || !PyDict_Check(a[1])) {
@@ -509,6 +729,7 @@ PyObject* setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
 #define PTO_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {PTO_METHOD(setup), PTO_METHOD(li_decode), PTO_METHOD(li_decode_bf16), PTO_METHOD(sfa), PTO_METHOD(sfa_packed),
                            PTO_METHOD(fused), PTO_METHOD(fused_bf16), PTO_METHOD(prolog_quant), PTO_METHOD(prolog),
+                           PTO_METHOD(qk_norm_rope), PTO_METHOD(kv_cache_write), PTO_METHOD(kv_cache_read), PTO_METHOD(prompt_attention),
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

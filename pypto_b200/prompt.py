@@ -19,7 +19,7 @@ import torch
 from . import _lib
 from .compat import Tensor as _Handle
 from .compat import unwrap
-from .ops import _need, _same_device, _workspace
+from .ops import _native, _need, _same_device, _workspace
 
 _ROW_DTYPES = {torch.bfloat16: _lib.PTO_DT_BF16, torch.float16: _lib.PTO_DT_F16}
 _LAYOUTS = {"half": _lib.PTO_ROPE_HALF, "interleaved": _lib.PTO_ROPE_INTERLEAVED, "deinterleave": _lib.PTO_ROPE_DEINTERLEAVE}
@@ -123,6 +123,10 @@ def qk_norm_rope(query, key, positions, rotary, query_out, key_out, *, query_wei
     [dk]. Head dims: multiples of 8 up to 256. `layout`: "half" pairs x[i] with x[i + r/2], "interleaved" x[2i] with x[2i + 1],
     "deinterleave" reads the second and writes the first (what the prologs do to the latent path's rope dims). The rotated dims are
     the head's first, or its last with `rope_last`. Sums and angles in fp32 and wider, one rounding at the end."""
+    if _native is not None and type(rotary) is RotaryFrequencies and layout in _LAYOUTS and _native.qk_norm_rope(
+            query, key, positions, rotary.turns, query_out, key_out, query_weight, key_weight, eps, _LAYOUTS[layout],
+            1 if rope_last else 0, rotary.rotary_dim, rotary.amplitude):
+        return None
     q = _rows(query, "query", 3)
     t, hq, dq = q.shape
     qo = _rows(query_out, "query_out", 3)
@@ -203,6 +207,9 @@ def kv_cache_write(key_nope, key_rope, cache_index, key_nope_2d, key_rope_2d, k_
     k_nope_scales float32 or float16 [rows, width/128], and / or `packed_kv_cache` int8 [rows, 656]: the caches that
     `sparse_flash_attention_quant_d/_p` and `sparse_attention_antiquant_d/_p` read. An index outside the cache is skipped and sets
     PTO_ST_BAD_PAGE in the workspace's status."""
+    if _native is not None and _native.kv_cache_write(key_nope, key_rope, cache_index, key_nope_2d, key_rope_2d, k_nope_scales,
+                                                      packed_kv_cache):
+        return None
     x = _rows(key_nope, "key_nope", 2)
     t, width = x.shape
     _need(width >= 128 and width % 128 == 0, "key_nope: [t, width], width a multiple of 128")
@@ -234,6 +241,9 @@ def kv_cache_read(key_nope_2d, key_rope_2d, k_nope_scales, block_table, cu_seqle
     block_table int32 [b, max_blocks], cu_seqlens int32 [b + 1] (from 0, not decreasing); key_nope_out bfloat16 or float16 [n, width],
     key_rope_out bfloat16 [n, 64] or None (not read); caches as in `kv_cache_write`, one of the two forms. Rows behind the last
     sequence are left as they are. A position without a valid page is written as zeros and sets PTO_ST_BAD_PAGE."""
+    if _native is not None and _native.kv_cache_read(key_nope_2d, key_rope_2d, k_nope_scales, block_table, cu_seqlens, key_nope_out,
+                                                     key_rope_out, block_size, first, packed_kv_cache):
+        return None
     out = _rows(key_nope_out, "key_nope_out", 2)
     n, width = out.shape
     _need(width >= 128 and width % 128 == 0, "key_nope_out: [n, width], width a multiple of 128")
@@ -278,6 +288,9 @@ def prompt_attention(query, key, value, cu_seqlens_q, cu_seqlens_k, attention_ou
     [b + 1]: where the sequences begin, from 0, not decreasing; rows of the output behind the last sequence are left as they are.
     softmax_scale positive, by default dqk^-0.5. `lse_out` (float32 [hq, tq], optional) receives ln sum exp of the scaled scores, with
     which results over different keys can be joined. A token without a key gets zeros and -inf."""
+    if _native is not None and softmax_scale is not None and _native.prompt_attention(
+            query, key, value, cu_seqlens_q, cu_seqlens_k, attention_out, softmax_scale, 1 if causal else 0, lse_out):
+        return None
     q, k, v, out = _rows(query, "query", 3), _rows(key, "key", 3), _rows(value, "value", 3), _rows(attention_out, "attention_out", 3)
     tq, hq, dqk = q.shape
     tk, hkv, dv = v.shape
