@@ -5,7 +5,7 @@
 namespace pto {
 namespace {
 
-constexpr int kWarps = 8;           // per block, all three kernels
+constexpr int kWarps = 4;  // per block, all three kernels (with eight a block's last warp keeps more registers: 64 tokens 6.2 us for 5.4)
 constexpr int kPackedRow = 656;     // 512 int8 | 64 bf16 | 4 f32
 constexpr int kPackedNope = 512;
 constexpr int kPackedScales = 640;
@@ -80,8 +80,8 @@ __device__ __forceinline__ void rope_lane(const NormRopeSide& s, uint64_t positi
   }
 }
 
-template <typename T, int kLayout>
-__global__ void __launch_bounds__(kWarps * 32) norm_rope_kernel(const NormRopeParams p) {
+template <typename T, int kLayout, bool kNorm>
+__global__ void __launch_bounds__(kWarps * 32, kNorm ? 6 : 8) norm_rope_kernel(const NormRopeParams p) {
   const int lane = threadIdx.x & 31;
   int64_t w = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
   const int side = w >= p.side[0].warps ? 1 : 0;
@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(kWarps * 32) norm_rope_kernel(const NormRopePa
                                       : __ldg(reinterpret_cast<const int*>(p.positions) + token);
     rope_lane<T, kLayout>(s, static_cast<uint64_t>(pos), p.turns, p.amplitude, li, rb, rv, cs, sn);
   }
-  if (s.weight != nullptr && li < vecs) unpack8<T>(__ldg(reinterpret_cast<const uint4*>(s.weight) + li), wt);
+  if (kNorm && s.weight != nullptr && li < vecs) unpack8<T>(__ldg(reinterpret_cast<const uint4*>(s.weight) + li), wt);
   const bool second = kLayout == PTO_ROPE_HALF && li >= rb + rv / 2;
   const int partner = (lane & ~(s.lanes - 1)) | (rotated ? (second ? li - rv / 2 : li + rv / 2) : li);
   const float inv_d = 1.f / static_cast<float>(s.d);
@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(kWarps * 32) norm_rope_kernel(const NormRopePa
       float x[8];
       unpack8<T>(v[i], x);
       v[i] = load(now + kAhead * s.split);
-      if (s.weight != nullptr) {
+      if (kNorm && s.weight != nullptr) {
         float ss = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv_write_kernel(const KvWritePara
 
 // ---- rows back -------------------------------------------------------------------------------------------------
 // out[cu[i] + j] = row of position first[i] + j of sequence i. A lane of a warp looks up the cache row of one output row each
-// (search of the sequence, block table), then the warp moves the rows one by one, four at a time in flight.
+// (search of the sequence, block table), then the warp moves the rows one by one, eight at a time in flight.
 // int8 -> fp32 without a conversion: 2^23 + (q + 128) is a float whose low byte is q + 128.
 __device__ __forceinline__ void dequant16(const uint4& v, float scale, float (&x)[16]) {
   const uint32_t u[4] = {v.x ^ 0x80808080u, v.y ^ 0x80808080u, v.z ^ 0x80808080u, v.w ^ 0x80808080u};
@@ -256,7 +256,7 @@ __device__ __forceinline__ void dequant16(const uint4& v, float scale, float (&x
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kWarps * 32) kv_read_kernel(const KvReadParams p) {
+__global__ void __launch_bounds__(kWarps * 32, 6) kv_read_kernel(const KvReadParams p) {
   const int lane = threadIdx.x & 31;
   const int64_t base = (static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5)) * p.per_warp;
   if (base >= p.n) return;
@@ -289,14 +289,14 @@ __global__ void __launch_bounds__(kWarps * 32) kv_read_kernel(const KvReadParams
     }
   }
   const int64_t width = static_cast<int64_t>(p.groups) * 128;
-  constexpr int kAhead = 4;
+  constexpr int kAhead = 8;
   for (int chunk = 0; chunk < p.chunks; ++chunk) {
     const int g = chunk * 4 + (lane >> 3);
     const bool mine = g < p.groups;
     for (int r0 = 0; r0 < count; r0 += kAhead) {
-      uint4 v[kAhead], rp = make_uint4(0, 0, 0, 0);
+      uint4 v[kAhead], rp[kAhead / 4];
       float sc[kAhead];
-      long long row[kAhead];
+      long long row[kAhead], rrow[kAhead / 4];
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
         row[k] = r0 + k < count ? __shfl_sync(0xffffffffu, from, r0 + k) : -1;
@@ -314,12 +314,16 @@ __global__ void __launch_bounds__(kWarps * 32) kv_read_kernel(const KvReadParams
         }
       }
       const bool ropes = p.rope_out != nullptr && chunk == 0;
-      const int mr = r0 + (lane >> 3);  // the rope part of four rows at once
-      const long long rrow = __shfl_sync(0xffffffffu, from, min(mr, count - 1));
-      const bool rope = ropes && mr < count && rrow != -1;
-      if (rope && rrow >= 0) {
-        rp = p.packed != nullptr ? ld_row(p.packed + rrow * kPackedRow + kPackedNope + (lane & 7) * 16)
-                                 : ld_row(reinterpret_cast<const uint16_t*>(p.rope) + rrow * 64 + (lane & 7) * 8);
+#pragma unroll
+      for (int k = 0; k < kAhead / 4; ++k) {  // the rope part of four rows at once
+        const int r = r0 + 4 * k + (lane >> 3);
+        rrow[k] = __shfl_sync(0xffffffffu, from, min(r, count - 1));
+        if (!ropes || r >= count) rrow[k] = -1;
+        rp[k] = make_uint4(0, 0, 0, 0);
+        if (rrow[k] >= 0) {
+          rp[k] = p.packed != nullptr ? ld_row(p.packed + rrow[k] * kPackedRow + kPackedNope + (lane & 7) * 16)
+                                      : ld_row(reinterpret_cast<const uint16_t*>(p.rope) + rrow[k] * 64 + (lane & 7) * 8);
+        }
       }
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
@@ -331,23 +335,26 @@ __global__ void __launch_bounds__(kWarps * 32) kv_read_kernel(const KvReadParams
           for (int e = 0; e < 16; ++e) x[e] = 0.f;
         }
         T* dst = reinterpret_cast<T*>(p.out) + (base + r0 + k) * p.out_ld + chunk * 512 + lane * 16;
-        uint4 lo, hi;
-        lo = make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
-        hi = make_uint4(pack2<T>(x[8], x[9]), pack2<T>(x[10], x[11]), pack2<T>(x[12], x[13]), pack2<T>(x[14], x[15]));
-        reinterpret_cast<uint4*>(dst)[0] = lo;
-        reinterpret_cast<uint4*>(dst)[1] = hi;
+        __stcs(reinterpret_cast<uint4*>(dst), make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7])));
+        __stcs(reinterpret_cast<uint4*>(dst) + 1,
+               make_uint4(pack2<T>(x[8], x[9]), pack2<T>(x[10], x[11]), pack2<T>(x[12], x[13]), pack2<T>(x[14], x[15])));
       }
-      if (rope) *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.rope_out) + (base + mr) * p.rope_out_ld + (lane & 7) * 8) = rp;
+#pragma unroll
+      for (int k = 0; k < kAhead / 4; ++k) {
+        if (rrow[k] == -1) continue;
+        const int r = r0 + 4 * k + (lane >> 3);
+        *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.rope_out) + (base + r) * p.rope_out_ld + (lane & 7) * 8) = rp[k];
+      }
     }
   }
 }
 
-template <typename T>
+template <typename T, bool kNorm>
 cudaError_t norm_rope(const NormRopeParams& p, int layout, unsigned grid, cudaStream_t stream) {
   switch (layout) {
-    case PTO_ROPE_HALF: norm_rope_kernel<T, PTO_ROPE_HALF><<<grid, kWarps * 32, 0, stream>>>(p); break;
-    case PTO_ROPE_INTERLEAVED: norm_rope_kernel<T, PTO_ROPE_INTERLEAVED><<<grid, kWarps * 32, 0, stream>>>(p); break;
-    default: norm_rope_kernel<T, PTO_ROPE_DEINTERLEAVE><<<grid, kWarps * 32, 0, stream>>>(p); break;
+    case PTO_ROPE_HALF: norm_rope_kernel<T, PTO_ROPE_HALF, kNorm><<<grid, kWarps * 32, 0, stream>>>(p); break;
+    case PTO_ROPE_INTERLEAVED: norm_rope_kernel<T, PTO_ROPE_INTERLEAVED, kNorm><<<grid, kWarps * 32, 0, stream>>>(p); break;
+    default: norm_rope_kernel<T, PTO_ROPE_DEINTERLEAVE, kNorm><<<grid, kWarps * 32, 0, stream>>>(p); break;
   }
   return cudaGetLastError();
 }
@@ -371,8 +378,10 @@ cudaError_t launch_norm_rope(const NormRopeParams& p, int dtype, int layout, cud
   const int64_t warps = p.side[0].warps + p.side[1].warps;
   if (warps == 0) return cudaSuccess;
   const unsigned grid = static_cast<unsigned>((warps + kWarps - 1) / kWarps);
+  const bool norm = p.side[0].weight != nullptr || p.side[1].weight != nullptr;
   count_launch();
-  return dtype == PTO_DT_BF16 ? norm_rope<__nv_bfloat16>(p, layout, grid, stream) : norm_rope<__half>(p, layout, grid, stream);
+  if (dtype == PTO_DT_BF16) return norm ? norm_rope<__nv_bfloat16, true>(p, layout, grid, stream) : norm_rope<__nv_bfloat16, false>(p, layout, grid, stream);
+  return norm ? norm_rope<__half, true>(p, layout, grid, stream) : norm_rope<__half, false>(p, layout, grid, stream);
 }
 
 cudaError_t launch_kv_write(const KvWriteParams& p, int dtype, cudaStream_t stream) {
