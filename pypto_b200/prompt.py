@@ -70,6 +70,15 @@ class RotaryFrequencies:
         bits = [round(f / (2 * math.pi) * 2.0 ** 64) for f in self.inv_freq]
         self.turns = torch.tensor([b - (1 << 64) if b >= 1 << 63 else b for b in bits], dtype=torch.int64, device=device)
 
+    @classmethod
+    def of(cls, turns, amplitude=1.0):
+        """From a tensor of turns made before (`turns` int64 [rotary_dim / 2])."""
+        _need(turns.dtype == torch.int64 and turns.dim() == 1 and turns.shape[0] >= 8 and turns.shape[0] % 8 == 0,
+              "turns: int64 [rotary_dim / 2]")
+        self = cls.__new__(cls)
+        self.rotary_dim, self.inv_freq, self.amplitude, self.turns = 2 * turns.shape[0], None, float(amplitude), turns
+        return self
+
 
 def _frequencies(r, base, scaling):
     """Angles a position of the r/2 pairs (Python floats) and the factor on cos and sin."""

@@ -17,10 +17,12 @@ this implementation reads, so they are not part of the op schemas).
 """
 from __future__ import annotations
 
+from typing import Optional
+
 import torch
 from torch import Tensor
 
-from . import ops
+from . import ops, prompt
 
 _NS = "pypto_b200"
 
@@ -125,12 +127,42 @@ def mla_indexer_prolog(token_x: Tensor, w_dq: Tensor, w_uq_qr: Tensor, w_uk: Ten
                            query_nope_out, query_rope_out, idx_query_out, idx_weights_out, epsilon_cq, epsilon_ckv)
 
 
+@torch.library.custom_op(f"{_NS}::qk_norm_rope", mutates_args=("query_out", "key_out"))
+def qk_norm_rope(query: Tensor, key: Optional[Tensor], positions: Tensor, turns: Tensor, query_out: Tensor,
+                 key_out: Optional[Tensor], query_weight: Optional[Tensor], key_weight: Optional[Tensor], amplitude: float = 1.0,
+                 eps: float = 1e-6, layout: str = "half", rope_last: bool = False) -> None:
+    """`turns`, `amplitude`: those of a `RotaryFrequencies`. Outputs apart from the inputs (an input written in place has no place in a
+    schema that names what is written)."""
+    prompt.qk_norm_rope(query, key, positions, prompt.RotaryFrequencies.of(turns, amplitude), query_out, key_out,
+                        query_weight=query_weight, key_weight=key_weight, eps=eps, layout=layout, rope_last=rope_last)
+
+
+@torch.library.custom_op(f"{_NS}::kv_cache_write", mutates_args=("key_nope_2d", "key_rope_2d", "k_nope_scales", "packed_kv_cache"))
+def kv_cache_write(key_nope: Tensor, key_rope: Optional[Tensor], cache_index: Tensor, key_nope_2d: Optional[Tensor],
+                   key_rope_2d: Optional[Tensor], k_nope_scales: Optional[Tensor], packed_kv_cache: Optional[Tensor] = None) -> None:
+    prompt.kv_cache_write(key_nope, key_rope, cache_index, key_nope_2d, key_rope_2d, k_nope_scales, packed_kv_cache=packed_kv_cache)
+
+
+@torch.library.custom_op(f"{_NS}::kv_cache_read", mutates_args=("key_nope_out", "key_rope_out"))
+def kv_cache_read(key_nope_2d: Optional[Tensor], key_rope_2d: Optional[Tensor], k_nope_scales: Optional[Tensor], block_table: Tensor,
+                  cu_seqlens: Tensor, key_nope_out: Tensor, key_rope_out: Optional[Tensor], block_size: int = 128,
+                  first: Optional[Tensor] = None, packed_kv_cache: Optional[Tensor] = None) -> None:
+    prompt.kv_cache_read(key_nope_2d, key_rope_2d, k_nope_scales, block_table, cu_seqlens, key_nope_out, key_rope_out, block_size,
+                         first=first, packed_kv_cache=packed_kv_cache)
+
+
+@torch.library.custom_op(f"{_NS}::prompt_attention", mutates_args=("attention_out", "lse_out"))
+def prompt_attention(query: Tensor, key: Tensor, value: Tensor, cu_seqlens_q: Tensor, cu_seqlens_k: Tensor, attention_out: Tensor,
+                     softmax_scale: float, causal: bool = True, lse_out: Optional[Tensor] = None) -> None:
+    prompt.prompt_attention(query, key, value, cu_seqlens_q, cu_seqlens_k, attention_out, softmax_scale, causal=causal, lse_out=lse_out)
+
+
 def _no_result(*args, **kwargs) -> None:
     return None
 
 
 OPS = (lightning_indexer_decode, sparse_flash_attention_quant, sparse_attention_antiquant,
        decode_indexer_attention_quant, lightning_indexer_topk_nonquant, decode_indexer_attention,
-       mla_indexer_prolog_quant, mla_indexer_prolog)
+       mla_indexer_prolog_quant, mla_indexer_prolog, qk_norm_rope, kv_cache_write, kv_cache_read, prompt_attention)
 for _op in OPS:
     _op.register_fake(_no_result)
