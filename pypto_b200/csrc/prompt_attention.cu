@@ -162,6 +162,7 @@ __device__ __forceinline__ int tile_keys(const PaParams& p, const PaTile& t) {  
 }
 
 constexpr int kBuckets = 256;
+constexpr int kPieceCost = 4, kCutCost = 4;
 struct PlanScratch {
   long long sum[32];
   int scan[32];
@@ -227,43 +228,67 @@ __device__ void build_table(const PaParams& p, PaHead* head, PaTile* tile, int* 
   sum = block_sum64(sum, s->sum) * p.hkv;
   longest = block_max(longest, s->scan);
 
-  // Pieces of at most `piece` key tiles. Where that evens out, no more pieces than CTAs: the shortest ones of which there are no more.
-  // Otherwise a third of a CTA's share each, so that the last ones to finish are not far apart (a piece costs a CTA about two tiles'
-  // time beside its keys; 16 sequences of 1 to 16384 keys x 8 heads in one wave: 117 us, in thirds PA_T16).
+  // Pieces of at most `piece` key tiles, every one of which costs a CTA about kPieceCost tiles' time beside its keys, and kCutCost more
+  // where its results are partial. Where there are
+  // fewer items than CTAs (they go round, in order): the shortest pieces of which there are no more than CTAs, or shorter ones in
+  // several rounds, whichever ends first. More items are handed out as CTAs become free: a long piece at the end leaves
+  // the others idle. (16 sequences of 1 to 16384 keys x 8 heads: one round 117 us, thirds of a CTA's share 98, this PA_T16.)
   int piece = max(longest, 1);
   if (p.slots > 0 && longest > kPaMinPiece) {
-    const int share = static_cast<int>((sum + ctas - 1) / ctas);
-    const int third = max((share + 2) / 3, kPaMinPiece);
-    if (static_cast<long long>(total) * p.hkv <= ctas && small) {
-      // each warp counts for a length of its own
-      int lo = kPaMinPiece, hi = longest;  // (as long as the longest: one piece each, which fits)
-      while (lo < hi) {
-        const int mid = lo + (hi - lo) * warp / warps;
-        int all = 0;
-        for (int t = lane; t < total; t += 32) all += max((s->n[t] + mid - 1) / mid, 1);
-        all = __reduce_add_sync(0xffffffffu, all);
-        __syncthreads();
-        if (lane == 0) s->scan[warp] = all * p.hkv <= ctas ? mid : INT_MAX;
-        __syncthreads();
-        // the shortest that fits, and the longest below it that does not
-        const int fits = static_cast<int>(__reduce_min_sync(0xffffffffu, static_cast<unsigned>(lane < warps ? s->scan[lane] : INT_MAX)));
-        const int mine_mid = lo + (hi - lo) * lane / warps;
-        const int fails = static_cast<int>(__reduce_max_sync(0xffffffffu, lane < warps && s->scan[min(lane, warps - 1)] == INT_MAX ? mine_mid : 0));
-        hi = min(hi, fits);
-        lo = max(lo, min(fails + 1, hi));
+    const long long share = (sum + ctas - 1) / ctas;
+    if (small) {
+      const bool rounds = static_cast<long long>(total) * p.hkv <= ctas;
+      const auto count = [&](int len, int& slots) {  // pieces of a head; called by a warp
+        int all = 0, cut = 0;
+        for (int t = lane; t < total; t += 32) {
+          const int k = max((s->n[t] + len - 1) / len, 1);
+          all += k;
+          cut += k > 1 ? k : 0;
+        }
+        slots = __reduce_add_sync(0xffffffffu, cut);
+        return __reduce_add_sync(0xffffffffu, all);
+      };
+      int lo = longest;
+      if (rounds) {  // each warp counts for a length of its own
+        int hi = longest, slots;
+        lo = kPaMinPiece;  // (as long as the longest: one piece each, which fits)
+        while (lo < hi) {
+          const int mid = lo + (hi - lo) * warp / warps;
+          const int all = count(mid, slots);
+          __syncthreads();
+          if (lane == 0) s->scan[warp] = all * p.hkv <= ctas ? mid : INT_MAX;
+          __syncthreads();
+          // the shortest that fits, and the longest below it that does not
+          const int fits = static_cast<int>(__reduce_min_sync(0xffffffffu, static_cast<unsigned>(lane < warps ? s->scan[lane] : INT_MAX)));
+          const int mine_mid = lo + (hi - lo) * lane / warps;
+          const int fails = static_cast<int>(__reduce_max_sync(0xffffffffu, lane < warps && s->scan[min(lane, warps - 1)] == INT_MAX ? mine_mid : 0));
+          hi = min(hi, fits);
+          lo = max(lo, min(fails + 1, hi));
+        }
       }
-      piece = lo <= share + share / 4 + 1 ? lo : third;
-    } else if (longest > 2 * third) {
-      piece = third;
+      // 32 lengths from a quarter of a share to two, and the one above
+      long long best = LLONG_MAX;
+      for (int j = warp; j <= 32; j += warps) {
+        const int len = j == 32 ? lo : static_cast<int>(max(static_cast<long long>(kPaMinPiece), share * (j + 4) / 16));
+        if (len > longest) continue;
+        int slots;
+        const long long all = static_cast<long long>(count(len, slots)) * p.hkv;
+        const long long cost = rounds ? (all + ctas - 1) / ctas * (len + kPieceCost + (slots > 0 ? kCutCost : 0)) * 2
+                                      : 2 * (sum + all * kPieceCost + static_cast<long long>(slots) * p.hkv * kCutCost) / ctas + len;
+        if (static_cast<long long>(slots) * p.hkv <= p.slots) best = min(best, cost << 24 | len);  // (below 2^24 tiles)
+      }
+      __syncthreads();
+      if (lane == 0) s->sum[warp] = best;
+      __syncthreads();
+      for (int i = 0; i < warps; ++i) best = min(best, s->sum[i]);
+      if (best != LLONG_MAX) piece = static_cast<int>(best & 0xffffff);
+    } else {
+      const int third = static_cast<int>(max((share + 2) / 3, static_cast<long long>(kPaMinPiece)));
+      if (longest > 2 * third && 2 * sum / third <= p.slots) piece = third;
     }
   }
-  if (piece < longest) {  // (the workspace is counted so that they fit)
-    const int k = (n + piece - 1) / piece;
-    const long long slots = small ? block_sum64(k > 1 ? k : 0, s->sum) * p.hkv : 2 * sum / piece;
-    if (slots > p.slots) piece = longest;
-  }
 
-  int pieces_all = 0, slots_all = 0;
+  int pieces_all = 0, slots_all = 0, cut = 0;  // cut: tiles up to the last one in pieces
   if (small) {
     if (tid < total) {
       int rank = 0;
@@ -297,6 +322,7 @@ __device__ void build_table(const PaParams& p, PaHead* head, PaTile* tile, int* 
     int all, all_slots;
     const int at = block_exclusive(c, s->scan, &all);
     const int at_slot = block_exclusive(c > 1 ? c : 0, s->scan, &all_slots);
+    cut = max(cut, block_max(c > 1 ? t + 1 : 0, s->scan));
     if (t < total) {
       tile[t].piece = pieces_all + at;
       tile[t].slot = c > 1 ? slots_all + at_slot : -1;
@@ -304,7 +330,7 @@ __device__ void build_table(const PaParams& p, PaHead* head, PaTile* tile, int* 
     pieces_all += all;
     slots_all += all_slots;
   }
-  if (tid == 0) *head = PaHead{total, pieces_all, 0, 0};
+  if (tid == 0) *head = PaHead{total, pieces_all, 0, cut};
   __syncthreads();
 }
 
@@ -1085,38 +1111,46 @@ __global__ void __launch_bounds__(256) pa_merge_kernel(const PaParams p) {
   const PaHead* head = reinterpret_cast<const PaHead*>(p.tables);
   const PaTile* tile = reinterpret_cast<const PaTile*>(head + 1);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long work = static_cast<long long>(head->tiles) * p.hkv;
+  const int chunks = (p.slot_rows + 7) / 8;  // of rows: a block takes eight
+  const long long work = static_cast<long long>(head->cut) * p.hkv * chunks;
   for (long long w = blockIdx.x; w < work; w += gridDim.x) {
-    const PaTile t = tile[w / p.hkv];
+    const long long item = w / chunks;
+    const PaTile t = tile[item / p.hkv];
     if (t.pieces <= 1) continue;
-    const int hk = static_cast<int>(w % p.hkv);
+    const int hk = static_cast<int>(item % p.hkv);
     const int rows = min(kPaRows, t.lq * p.group - t.row0);
     const int64_t slot = static_cast<int64_t>(t.slot) * p.hkv + hk * t.pieces;
-    for (int row = warp; row < rows; row += 8) {
+    if (const int row = static_cast<int>(w - item * chunks) * 8 + warp; row < rows) {
       float top = -INFINITY;
       for (int i = lane; i < t.pieces; i += 32) top = fmaxf(top, p.part_ml[(slot + i) * p.slot_rows + row].x);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
       float y[kPer] = {}, all = 0.f;
-#pragma unroll 4
-      for (int i = 0; i < t.pieces; ++i) {
-        const float2 ml = p.part_ml[(slot + i) * p.slot_rows + row];
-        if (ml.x == -INFINITY) continue;
-        const float f = ex2f(ml.x - top);
-        all += ml.y * f;
-        const float* src = p.part_o + ((slot + i) * p.slot_rows + row) * DV + lane * kPer;
-        if constexpr (kPer == 4) {
-          const float4 v = *reinterpret_cast<const float4*>(src);
-          y[0] = fmaf(v.x, f, y[0]);
-          y[1] = fmaf(v.y, f, y[1]);
-          y[2] = fmaf(v.z, f, y[2]);
-          y[3] = fmaf(v.w, f, y[3]);
-        } else {
-          const float2 v = *reinterpret_cast<const float2*>(src);
-          y[0] = fmaf(v.x, f, y[0]);
-          y[1] = fmaf(v.y, f, y[1]);
+      for (int i0 = 0; i0 < t.pieces; i0 += 32) {
+        // a lane's piece: its weight (0 where it has seen no key), its sum
+        const float2 ml = i0 + lane < t.pieces ? p.part_ml[(slot + i0 + lane) * p.slot_rows + row] : make_float2(-INFINITY, 0.f);
+        const float weight = ml.x == -INFINITY ? 0.f : ex2f(ml.x - top);
+        all += ml.x == -INFINITY ? 0.f : ml.y * weight;
+        const int n = min(32, t.pieces - i0);
+        const float* src = p.part_o + ((slot + i0) * p.slot_rows + row) * DV + lane * kPer;
+        const int64_t step = static_cast<int64_t>(p.slot_rows) * DV;
+#pragma unroll 8
+        for (int i = 0; i < n; ++i) {
+          const float f = __shfl_sync(0xffffffffu, weight, i);
+          float v[kPer];
+          if constexpr (kPer == 4) {
+            const float4 q = __ldcg(reinterpret_cast<const float4*>(src + i * step));
+            v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
+          } else {
+            const float2 q = __ldcg(reinterpret_cast<const float2*>(src + i * step));
+            v[0] = q.x, v[1] = q.y;
+          }
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) y[e] = f != 0.f ? fmaf(v[e], f, y[e]) : y[e];
         }
       }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
       const float inv = all == 0.f ? 0.f : 1.f / all;
       const int tok = row_token(p, t.row0 + row);
       const int h = hk * p.group + t.row0 + row - tok * p.group;
@@ -1148,7 +1182,7 @@ cudaError_t launch(const PaParams& p, const void* tmap_q, const void* tmap_k, co
   if (e != cudaSuccess) return e;
   count_launch();
   if (p.slots > 0) {
-    e = launch_maybe_pdl(pa_merge_kernel<DV, F16>, dim3(ctas * 2), dim3(256), 0, stream, true, p);
+    e = launch_maybe_pdl(pa_merge_kernel<DV, F16>, dim3(ctas * 6), dim3(256), 0, stream, true, p);
     count_launch();
   }
   return e;

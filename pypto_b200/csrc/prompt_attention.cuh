@@ -20,7 +20,7 @@ struct alignas(16) PaTile {
 struct PaHead {
   int tiles, pieces;  // of the table
   int next;           // items handed out beyond the first ones
-  int pad;
+  int cut;            // tiles up to the last one that is in several pieces
 };
 
 struct PaParams {
