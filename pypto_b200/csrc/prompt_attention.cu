@@ -841,16 +841,24 @@ __device__ __forceinline__ void role_softmax(const PaParams& p, const Ctx& x, in
       wait_bar(c, sfull + (ns & 1) * 8, (ns >> 1) & 1, p.status, 93);
       __syncwarp();
       tc_fence_after();
+      if (key0 + (k + 1) * C::kStep > sure) {  // hidden keys: into the scores' columns, so that the way without any has no code for it
+        const int left = limit - (key0 + k * C::kStep);
+#pragma unroll 1
+        for (int h = 0; h < C::kStep / 32; ++h) {
+          uint32_t o[32];
+          tmem_ld_32x32b_x32(t_s + 32 * h, o);
+          tc_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 32 * h + i < left ? o[i] : 0xff800000u;
+          tmem_st_32x32b_x32(t_s + 32 * h, o);
+        }
+        tc_wait_st();
+      }
       uint32_t u[C::kStep / 32][32];
       float(&v)[C::kStep / 32][32] = reinterpret_cast<float(&)[C::kStep / 32][32]>(u);
 #pragma unroll
       for (int h = 0; h < C::kStep / 32; ++h) tmem_ld_32x32b_x32(t_s + 32 * h, u[h]);
       tc_wait_ld();
-      const int left = limit - (key0 + k * C::kStep);
-      if (key0 + (k + 1) * C::kStep > sure) {
-#pragma unroll
-        for (int i = 0; i < C::kStep; ++i) v[i >> 5][i & 31] = i < left ? v[i >> 5][i & 31] : -INFINITY;
-      }
       float top[C::kStep / 16];
 #pragma unroll
       for (int h = 0; h < C::kStep / 16; ++h) {
