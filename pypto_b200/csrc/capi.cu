@@ -1440,7 +1440,8 @@ int pto_prompt_attention(const void* query, const void* key, const void* value, 
   // key heads worked on together: as many as half of L2 holds the keys and values of
   const int64_t head_bytes = static_cast<int64_t>(tk) * (dqk + dv) * 2;
   const int64_t set = head_bytes > 0 ? (64ll << 20) / head_bytes : hkv;
-  p.head_set = static_cast<int>(set < 1 ? 1 : set > hkv ? hkv : set);
+  const int64_t sets = set < 1 ? hkv : (hkv + set - 1) / set;  // of equal size: a small last one would leave CTAs idle
+  p.head_set = static_cast<int>((hkv + sets - 1) / sets);
   p.scale = softmax_scale;
   p.scale_log2 = softmax_scale * 1.44269504088896340736f;
   p.max_tiles = w.max_tiles;

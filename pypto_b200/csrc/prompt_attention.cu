@@ -531,6 +531,17 @@ __device__ __forceinline__ void role_queries(const PaParams& p, const Ctx& x, co
     if (p.q_map) {
       // rows are token-major, so a tile is a box of 128 / group tokens x group heads; what lies behind the sequence is not written
       const int token = q0 + row_token(p, row0);
+      if (n_item > 0 && elect_one()) {  // into L2 while the tiles are still read
+        for (int s = 0; s < (dual ? 1 : 2); ++s) {
+#pragma unroll
+          for (int ch = 0; ch < DQK / 64; ++ch) {
+            asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global [%0, {%1, %2, %3}];" ::"l"(mq), "r"(ch * 64), "r"(head),
+                         "r"(token + (s == 1 ? row_token(p, 128) : 0))
+                         : "memory");
+          }
+        }
+      }
+      __syncwarp();
       for (int s = 0; s < 2; ++s) {
         if (n_item > 0) wait_warp(c, c->qempty[s], (n_item - 1) & 1, p.status, 83);
         if (elect_one() && !*reinterpret_cast<volatile int*>(&c->expired)) {
