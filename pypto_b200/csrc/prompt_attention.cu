@@ -5,10 +5,12 @@
 // against its keys: two MMA tiles of 128 rows, two streams, and every K and V tile that is loaded serves both. A stream goes in
 // steps of 64 keys. TMEM holds the scores of two steps of each stream, whose first half the probabilities overwrite as 16-bit
 // values (the A operand of the value product from there), and both outputs; the scores of step i + 2 follow the value product of
-// step i, so the softmax finds the next step's scores ready while the tensor pipe works on the ones before. (Steps of 128 keys
-// in one buffer: the pipe waited for the softmax and the softmax for it, 8192 tokens x 32 heads 490 us; in buffers of their own for
-// scores and probabilities, two hand-overs a step, 505. Score products of 64 keys take the pipe 48 cycles instead of 32: shared
-// memory delivers 128 bytes a cycle.)
+// step i, so the softmax finds the next step's scores ready while the tensor pipe works on the ones before. Measured on 8192 tokens x
+// 32 heads on 8 key heads of 128, causal: 462 us, 1190 TFLOP/s (72 % of the GEMM's burst rate; under the power cap of a long run 541).
+// Steps of 128 keys in one buffer, probabilities handed over by halves: the pipe waits for the softmax and the softmax for it, 497;
+// scores and probabilities of 64 keys in columns of their own, two hand-overs a step: 505, where this had 485. What bounds it is shared
+// memory, which delivers 128 bytes a cycle: score products of 64 keys take 48 cycles instead of 32, and without any softmax at all
+// the kernel still takes 401 us.
 // An item of at most 128 rows (a few tokens, single ones) has one tile; both streams take it, each with half of the keys, and the
 // halves are merged at the end.
 // Warps: 0 and 1 issue the MMAs of stream 0 and 1, 2 hands out items and loads K and V by TMA through a ring, 3 loads queries and
@@ -40,7 +42,8 @@ struct Cfg {
   // f16 probabilities are kept away from its subnormal values: times 2^4 (a maximum that lags by 2^8 leaves them below 2^12)
   static constexpr float kBias = F16 ? 4.f : 0.f;
 };
-constexpr int kFmaPairs = 1;  // of eight pairs of probabilities, those whose exponentials the FMA pipe computes
+// Of eight pairs of probabilities, those whose exponentials the FMA pipe computes (8192 tokens, 0 to 3 of eight: 480, 462, 469, 472 us)
+constexpr int kFmaPairs = 1;
 constexpr float kLag = 8.f;  // a maximum is raised, and the output rescaled, once it is 2^8 behind
 
 struct alignas(16) Item {
@@ -232,7 +235,7 @@ __device__ void build_table(const PaParams& p, PaHead* head, PaTile* tile, int* 
   // where its results are partial. Where there are
   // fewer items than CTAs (they go round, in order): the shortest pieces of which there are no more than CTAs, or shorter ones in
   // several rounds, whichever ends first. More items are handed out as CTAs become free: a long piece at the end leaves
-  // the others idle. (16 sequences of 1 to 16384 keys x 8 heads: one round 117 us, thirds of a CTA's share 98, this PA_T16.)
+  // the others idle. (16 sequences of 1 to 16384 keys x 8 heads: one round 117 us, thirds of a CTA's share 98, this 94.)
   int piece = max(longest, 1);
   if (p.slots > 0 && longest > kPaMinPiece) {
     const long long share = (sum + ctas - 1) / ctas;
@@ -774,8 +777,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 // 2^x of a pair on the FMA pipe: x = n + f, |f| <= 1/2, n from the sum with 1.5 * 2^23; 2^f by the polynomial of degree four with
 // p(0) = 1 and the smallest relative error on that interval (2.8e-6; computed by Lawson's iteration); n goes to the exponent. 0 for
-// x <= -127. The exponential unit gives 16 values a clock and SM, half of what the products of a tile take: a share of
-// the exponentials goes this way.
+// x <= -127. The exponential unit gives 16 values a clock and SM, so a tile's take as long as its products: a share of them goes
+// this way.
 template <int N, int M>
 __device__ __forceinline__ void exp2_fma(float2 (&x)[M]) {  // of the first N pairs
   float2 t[N > 0 ? N : 1], y[N > 0 ? N : 1];
@@ -1140,15 +1143,17 @@ __global__ void __launch_bounds__(256) pa_merge_kernel(const PaParams p) {
     const int rows = min(kPaRows, t.lq * p.group - t.row0);
     const int64_t slot = static_cast<int64_t>(t.slot) * p.hkv + hk * t.pieces;
     if (const int row = static_cast<int>(w - item * chunks) * 8 + warp; row < rows) {
-      float top = -INFINITY;
-      for (int i = lane; i < t.pieces; i += 32) top = fmaxf(top, p.part_ml[(slot + i) * p.slot_rows + row].x);
+      // a lane's piece, of the first 32: its maximum and sum
+      const float2 own = lane < t.pieces ? p.part_ml[(slot + lane) * p.slot_rows + row] : make_float2(-INFINITY, 0.f);
+      float top = own.x;
+      for (int i = lane + 32; i < t.pieces; i += 32) top = fmaxf(top, p.part_ml[(slot + i) * p.slot_rows + row].x);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
       float y[kPer] = {}, all = 0.f;
       for (int i0 = 0; i0 < t.pieces; i0 += 32) {
-        // a lane's piece: its weight (0 where it has seen no key), its sum
-        const float2 ml = i0 + lane < t.pieces ? p.part_ml[(slot + i0 + lane) * p.slot_rows + row] : make_float2(-INFINITY, 0.f);
-        const float weight = ml.x == -INFINITY ? 0.f : ex2f(ml.x - top);
+        float2 ml = own;
+        if (i0 > 0) ml = i0 + lane < t.pieces ? p.part_ml[(slot + i0 + lane) * p.slot_rows + row] : make_float2(-INFINITY, 0.f);
+        const float weight = ml.x == -INFINITY ? 0.f : ex2f(ml.x - top);  // (0: it has seen no key)
         all += ml.x == -INFINITY ? 0.f : ml.y * weight;
         const int n = min(32, t.pieces - i0);
         const float* src = p.part_o + ((slot + i0) * p.slot_rows + row) * DV + lane * kPer;
@@ -1201,7 +1206,7 @@ cudaError_t launch(const PaParams& p, const void* tmap_q, const void* tmap_k, co
   if (e != cudaSuccess) return e;
   count_launch();
   if (p.slots > 0) {
-    e = launch_maybe_pdl(pa_merge_kernel<DV, F16>, dim3(ctas * 6), dim3(256), 0, stream, true, p);
+    e = launch_maybe_pdl(pa_merge_kernel<DV, F16>, dim3(ctas * 5), dim3(256), 0, stream, true, p);
     count_launch();
   }
   return e;

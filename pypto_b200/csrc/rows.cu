@@ -63,10 +63,11 @@ __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
 // mod 2^64, IS the fraction of a turn, exact at any position, where an angle in fp32 loses 1e-2 rad at 10^5. cos and sin of its
 // upper 32 bits are within 1e-7.
 // A lane holds eight neighbouring dims of a head, a power of two of lanes a head, so sums and the other half of a pair travel by
-// shuffles. A warp takes heads of ONE token: its lanes' cosines and sines (eight of each at most) are computed once and stay in
+// shuffles. With weights, cosines and sines multiplied beforehand a dim costs four operations besides its conversions; the kernel with a
+// norm is bound by instructions (16384 tokens x 40 heads: issue slots 76 % busy before that). A warp takes heads of ONE token: its lanes' cosines and sines (eight of each at most) are computed once and stay in
 // registers. With few tokens the heads of one are shared out over as many warps as fill the SMs.
-template <typename T, int kLayout>
-__device__ __forceinline__ void rope_lane(const NormRopeSide& s, uint64_t position, const uint64_t* __restrict__ turns, float amplitude,
+template <int kLayout>
+__device__ __forceinline__ void rope_lane(uint64_t position, const uint64_t* __restrict__ turns, float amplitude,
                                           int li, int rb, int rv, float (&cs)[8], float (&sn)[8]) {
   // half: dims 8*(li - rb) + e of a half; pairs side by side: pairs 4*(li - rb) + e
   const int first = kLayout == PTO_ROPE_HALF ? 8 * ((li - rb) % (rv / 2)) : 4 * (li - rb);
@@ -108,17 +109,37 @@ __global__ void __launch_bounds__(kWarps * 32, kNorm ? 6 : 8) norm_rope_kernel(c
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) v[i] = load(part + i * s.split);
 
-  float cs[8], sn[8], wt[8];
+  // What a dim is multiplied with and what the pair's other dim is, weights and angles in one; pairs side by side without weights need
+  // one of each a pair.
+  constexpr bool kHalf = kLayout == PTO_ROPE_HALF;
+  constexpr int kEach = kHalf || kNorm ? 8 : 4;
+  float mul[kEach], oth[kEach];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) wt[e] = cs[e] = 1.f, sn[e] = 0.f;
+  for (int e = 0; e < kEach; ++e) mul[e] = 1.f, oth[e] = 0.f;
+  const bool second = kHalf && li >= rb + rv / 2;
+  const int partner = (lane & ~(s.lanes - 1)) | (rotated ? (second ? li - rv / 2 : li + rv / 2) : li);
   if (rotated) {
     const int64_t pos = p.positions64 ? __ldg(reinterpret_cast<const long long*>(p.positions) + token)
                                       : __ldg(reinterpret_cast<const int*>(p.positions) + token);
-    rope_lane<T, kLayout>(s, static_cast<uint64_t>(pos), p.turns, p.amplitude, li, rb, rv, cs, sn);
+    float cs[8], sn[8];
+    rope_lane<kLayout>(static_cast<uint64_t>(pos), p.turns, p.amplitude, li, rb, rv, cs, sn);
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const int i = kHalf || kEach == 4 ? e : e >> 1;
+      mul[e] = cs[i];
+      oth[e] = (kHalf ? second : kEach == 4 || (e & 1) != 0) ? sn[i] : -sn[i];
+    }
   }
-  if (kNorm && s.weight != nullptr && li < vecs) unpack8<T>(__ldg(reinterpret_cast<const uint4*>(s.weight) + li), wt);
-  const bool second = kLayout == PTO_ROPE_HALF && li >= rb + rv / 2;
-  const int partner = (lane & ~(s.lanes - 1)) | (rotated ? (second ? li - rv / 2 : li + rv / 2) : li);
+  if (kNorm && li < vecs) {
+    float mine_w[8], other_w[8];
+    unpack8<T>(__ldg(reinterpret_cast<const uint4*>(s.weight) + li), mine_w);
+    unpack8<T>(__ldg(reinterpret_cast<const uint4*>(s.weight) + (kHalf ? partner & (s.lanes - 1) : li)), other_w);
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      mul[e] *= mine_w[e];
+      oth[e] *= other_w[kHalf ? e : e ^ 1];
+    }
+  }
   const float inv_d = 1.f / static_cast<float>(s.d);
 
   for (int st = part; st < steps; st += kAhead * s.split) {
@@ -126,44 +147,44 @@ __global__ void __launch_bounds__(kWarps * 32, kNorm ? 6 : 8) norm_rope_kernel(c
     for (int i = 0; i < kAhead; ++i) {
       const int now = st + i * s.split;
       if (now >= steps) break;
-      float x[8];
+      float x[8], y[8];
       unpack8<T>(v[i], x);
       v[i] = load(now + kAhead * s.split);
-      if (kNorm && s.weight != nullptr) {
+      if constexpr (kEach == 8) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float other = kHalf ? __shfl_sync(0xffffffffu, x[e], partner) : x[e ^ 1];
+          y[e] = fmaf(x[e], mul[e], other * oth[e]);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          y[2 * e] = fmaf(x[2 * e], mul[e], -x[2 * e + 1] * oth[e]);
+          y[2 * e + 1] = fmaf(x[2 * e + 1], mul[e], x[2 * e] * oth[e]);
+        }
+      }
+      if (kNorm) {
         float ss = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
         for (int o = s.lanes >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
         const float inv = rsqrtf(fmaf(ss, inv_d, p.eps));
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * wt[e];
+        for (int e = 0; e < 8; ++e) y[e] *= inv;
       }
       const int h = now * per + sub;
-      T* out = dst + h * s.out_head;
+      if (!kNorm) {  // a dim that is only copied is copied whatever it is (inf * 0 is not 0)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = rotated ? y[e] : x[e];
+      }
       const bool store = mine && h < s.heads;
-      if constexpr (kLayout == PTO_ROPE_HALF) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float other = __shfl_sync(0xffffffffu, x[e], partner);
-          x[e] = rotated ? fmaf(x[e], cs[e], second ? other * sn[e] : -other * sn[e]) : x[e];
-        }
-        if (store) *reinterpret_cast<uint4*>(out) = pack8<T>(x);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float a = x[2 * e], b = x[2 * e + 1];
-          if (rotated) {
-            x[2 * e] = fmaf(a, cs[e], -b * sn[e]);
-            x[2 * e + 1] = fmaf(a, sn[e], b * cs[e]);
-          }
-        }
-        if (kLayout == PTO_ROPE_INTERLEAVED || !rotated) {
-          if (store) *reinterpret_cast<uint4*>(out) = pack8<T>(x);
-        } else if (store) {  // the pairs' first values in the first half, their second ones in the second
-          T* lo = out - li * 8 + rb * 8 + (li - rb) * 4;
-          *reinterpret_cast<uint2*>(lo) = make_uint2(pack2<T>(x[0], x[2]), pack2<T>(x[4], x[6]));
-          *reinterpret_cast<uint2*>(lo + rv * 4) = make_uint2(pack2<T>(x[1], x[3]), pack2<T>(x[5], x[7]));
-        }
+      T* out = dst + h * s.out_head;
+      if (kLayout != PTO_ROPE_DEINTERLEAVE || !rotated) {
+        if (store) *reinterpret_cast<uint4*>(out) = pack8<T>(y);
+      } else if (store) {  // the pairs' first values in the first half, their second ones in the second
+        T* lo = out - li * 8 + rb * 8 + (li - rb) * 4;
+        *reinterpret_cast<uint2*>(lo) = make_uint2(pack2<T>(y[0], y[2]), pack2<T>(y[4], y[6]));
+        *reinterpret_cast<uint2*>(lo + rv * 4) = make_uint2(pack2<T>(y[1], y[3]), pack2<T>(y[5], y[7]));
       }
     }
   }
@@ -375,6 +396,17 @@ void norm_rope_plan(NormRopeSide* s, int64_t t, int num_sms) {
 }
 
 cudaError_t launch_norm_rope(const NormRopeParams& p, int dtype, int layout, cudaStream_t stream) {
+  if (p.side[0].warps > 0 && p.side[1].warps > 0 && (p.side[0].weight == nullptr) != (p.side[1].weight == nullptr)) {
+    for (int i = 0; i < 2; ++i) {  // a kernel with a norm and one without
+      NormRopeParams one = p;
+      one.side[0] = p.side[i];
+      one.side[1].warps = 0;
+      one.side[1].weight = nullptr;
+      const cudaError_t e = launch_norm_rope(one, dtype, layout, stream);
+      if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
+  }
   const int64_t warps = p.side[0].warps + p.side[1].warps;
   if (warps == 0) return cudaSuccess;
   const unsigned grid = static_cast<unsigned>((warps + kWarps - 1) / kWarps);

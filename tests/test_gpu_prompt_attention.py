@@ -114,6 +114,10 @@ def test_prompts(ql, kl, hq, hkv, dqk, dv, dtype):
     ([60], [9000], 5, 1, 192, 128, BF, True),
     ([40, 30], [10, 0], 4, 2, 128, 128, BF, True),  # tokens without a key
     ([0, 9, 0, 300, 0], [4, 9, 0, 100, 7], 6, 2, 64, 64, F16, True),
+    ([3, 200], [0, 0], 2, 1, 128, 128, BF, True),  # no keys at all
+    ([5, 0], [700, 900], 2, 2, 192, 128, F16, False),
+    ([255, 1, 513], [4000, 4000, 4000], 16, 1, 64, 64, BF, True),
+    ([1] * 40, [2500] * 40, 32, 8, 128, 128, BF, True),  # more items than one round
     ([50, 20], [300, 64], 4, 4, 128, 128, BF, False),
     ([600], [600], 7, 1, 128, 128, F16, True),  # groups that are no power of two
     ([33], [1000], 128, 1, 64, 64, BF, True),  # one key head for all

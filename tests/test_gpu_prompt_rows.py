@@ -119,6 +119,28 @@ def test_heads_first_storage_and_a_head_that_all_tokens_share():
     close_heads(ko, k, None, pos, rot, "interleaved", True)
 
 
+def test_dims_that_are_not_rotated_are_copied_whatever_they_are():
+    for layout, last in (("half", False), ("interleaved", True), ("deinterleave", True)):
+        x = rand(9, 2, 96, seed=30).to(DEV)
+        at = 5 if last else 90
+        x[4, 1, at], x[5, 0, at], x[6, 0, at + 1] = math.inf, -math.inf, math.nan
+        out = torch.empty_like(x)
+        pto.qk_norm_rope(x, None, torch.arange(9, device=DEV), pto.RotaryFrequencies(64), out, None, layout=layout, rope_last=last)
+        kept = slice(0, 32) if last else slice(64, 96)
+        assert torch.equal(out[..., kept].isnan(), x[..., kept].isnan())
+        assert torch.equal(out[..., kept].nan_to_num(3), x[..., kept].nan_to_num(3))
+        assert bool(out[..., 32:].isfinite().all() if last else out[..., :64].isfinite().all())
+
+
+def test_one_side_with_a_norm():
+    q, k = rand(50, 4, 128, seed=31).to(DEV), rand(50, 2, 128, seed=32).to(DEV)
+    w, pos, rot = rand(128, seed=33).to(DEV), torch.arange(50, device=DEV), pto.RotaryFrequencies(64)
+    qo, ko = torch.empty_like(q), torch.empty_like(k)
+    pto.qk_norm_rope(q, k, pos, rot, qo, ko, key_weight=w)
+    close_heads(qo, q, None, pos, rot, "half", False)
+    close_heads(ko, k, w, pos, rot, "half", False)
+
+
 def test_norm_alone_and_rows_of_zeros():
     x = rand(40, 4, 128, seed=11).to(DEV)
     x[3] = 0
