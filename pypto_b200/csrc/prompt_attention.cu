@@ -290,32 +290,47 @@ __device__ void build_table(const PaParams& p, PaHead* head, PaTile* tile, int* 
     }
   }
 
-  int pieces_all = 0, slots_all = 0, cut = 0;  // cut: tiles up to the last one in pieces
   if (small) {
+    // Every thread counts the pieces before its tile's: no scan, and nothing of the table is read back.
+    const auto pieces_of = [&](int k) { return max((k + piece - 1) / piece, 1); };
+    if (tid < total) s->first[tid] = mine.pieces = pieces_of(n);  // (the sequences' first tiles have been looked up)
+    __syncthreads();
+    int rank = 0, before = 0, slots_before = 0, all = 0, cut = 0;
+    for (int t = 0; t < total; ++t) {
+      const int k = s->n[t], c = s->first[t], many = c > 1 ? c : 0;
+      const bool ahead = k > n || (k == n && t < tid);
+      rank += ahead;
+      before += ahead ? c : 0;
+      slots_before += ahead ? many : 0;
+      all += c;
+      cut += many > 0;  // (the longest come first, and so do those in pieces)
+    }
     if (tid < total) {
-      int rank = 0;
-      for (int t = 0; t < total; ++t) rank += s->n[t] > n || (s->n[t] == n && t < tid);
-      mine.pieces = max((n + piece - 1) / piece, 1);
+      mine.piece = before;
+      mine.slot = mine.pieces > 1 ? slots_before : -1;
       tile[rank] = mine;
     }
-  } else {
-    const float per = static_cast<float>(kBuckets - 1) / static_cast<float>(max(longest, 1));
-    auto bucket = [&](int k) { return kBuckets - 1 - static_cast<int>(static_cast<float>(k) * per); };
-    for (int i = tid; i < kBuckets; i += nt) s->n[i] = 0;
+    if (tid == 0) *head = PaHead{total, all, 0, cut};
     __syncthreads();
-    for (int t = tid; t < total; t += nt) atomicAdd(&s->n[min(max(bucket(tile_keys(p, look(t))), 0), kBuckets - 1)], 1);
-    __syncthreads();
-    int all;
-    const int c = tid < kBuckets ? s->n[tid] : 0;
-    const int at = block_exclusive(c, s->scan, &all);
-    if (tid < kBuckets) s->n[tid] = at;
-    __syncthreads();
-    for (int t = tid; t < total; t += nt) {
-      PaTile x = look(t);
-      const int k = tile_keys(p, x);
-      x.pieces = max((k + piece - 1) / piece, 1);
-      tile[atomicAdd(&s->n[min(max(bucket(k), 0), kBuckets - 1)], 1)] = x;
-    }
+    return;
+  }
+  int pieces_all = 0, slots_all = 0, cut = 0;  // cut: tiles up to the last one in pieces
+  const float per = static_cast<float>(kBuckets - 1) / static_cast<float>(max(longest, 1));
+  auto bucket = [&](int k) { return kBuckets - 1 - static_cast<int>(static_cast<float>(k) * per); };
+  for (int i = tid; i < kBuckets; i += nt) s->n[i] = 0;
+  __syncthreads();
+  for (int t = tid; t < total; t += nt) atomicAdd(&s->n[min(max(bucket(tile_keys(p, look(t))), 0), kBuckets - 1)], 1);
+  __syncthreads();
+  int all;
+  const int c = tid < kBuckets ? s->n[tid] : 0;
+  const int at = block_exclusive(c, s->scan, &all);
+  if (tid < kBuckets) s->n[tid] = at;
+  __syncthreads();
+  for (int t = tid; t < total; t += nt) {
+    PaTile x = look(t);
+    const int k = tile_keys(p, x);
+    x.pieces = max((k + piece - 1) / piece, 1);
+    tile[atomicAdd(&s->n[min(max(bucket(k), 0), kBuckets - 1)], 1)] = x;
   }
   __syncthreads();
   for (int base = 0; base < total; base += nt) {
@@ -349,9 +364,9 @@ __global__ void __launch_bounds__(1024) pa_plan_kernel(const PaParams p, int cta
 __device__ __forceinline__ Item find_item(const PaParams& p, const PaTile* tile, int tiles, int pieces, long long w) {
   Item it = {};
   if (w >= static_cast<long long>(pieces) * p.hkv) return it;
-  const long long per_set = static_cast<long long>(pieces) * p.head_set;
-  const int set = static_cast<int>(w / per_set);
-  const int rem = static_cast<int>(w - set * per_set);  // (below pieces * heads: the host side refuses 2^31)
+  const unsigned per_set = static_cast<unsigned>(pieces) * p.head_set;  // (pieces * heads: the host side refuses 2^31)
+  const int set = static_cast<unsigned>(w) / per_set;
+  const int rem = static_cast<unsigned>(w) - set * per_set;
   const int heads = min(p.head_set, p.hkv - set * p.head_set);
   const int which = rem / heads;
   it.head = set * p.head_set + rem - which * heads;
