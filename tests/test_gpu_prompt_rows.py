@@ -119,6 +119,15 @@ def test_heads_first_storage_and_a_head_that_all_tokens_share():
     close_heads(ko, k, None, pos, rot, "interleaved", True)
 
 
+def test_pairs_taken_apart_in_place():
+    """Every lane writes dims that two others have read."""
+    pos, rot = torch.arange(333, device=DEV), pto.RotaryFrequencies(192)
+    x = rand(333, 9, 256, seed=31).to(DEV)
+    y = x.clone()
+    pto.qk_norm_rope(y, None, pos, rot, y, None, layout="deinterleave", rope_last=True)
+    close_heads(y, x, None, pos, rot, "deinterleave", True)
+
+
 def test_dims_that_are_not_rotated_are_copied_whatever_they_are():
     for layout, last in (("half", False), ("interleaved", True), ("deinterleave", True)):
         x = rand(9, 2, 96, seed=30).to(DEV)
