@@ -643,6 +643,7 @@ struct PaWs {
   int64_t table_stride;
   size_t tables, part_ml, part_o, total;
 };
+constexpr int kPaSequences = 1 << 24;  // of a call (its tiles are counted in 32 bits)
 PaWs pa_ws(int tq, int tk, int b, int hq, int hkv, int dv) {
   PaWs w{};
   const int group = hq / hkv;
@@ -1265,6 +1266,7 @@ int pto_qk_norm_rope(const void* query, const void* key, const void* positions, 
   PTO_REQUIRE(strides != nullptr, "strides is null");
   PTO_REQUIRE(rotary_dim >= 0 && rotary_dim % 16 == 0, "rotary_dim %d: a multiple of 16 expected", rotary_dim);
   PTO_REQUIRE(layout >= PTO_ROPE_HALF && layout <= PTO_ROPE_DEINTERLEAVE, "layout %d", layout);
+  PTO_REQUIRE(eps >= 0.f, "eps must not be negative");
   if (t == 0 || (hq == 0 && hk == 0)) return PTO_OK;
   PTO_REQUIRE(rotary_dim == 0 || (positions && turns), "null tensor pointer");
   pto::NormRopeParams p{};
@@ -1361,7 +1363,10 @@ int pto_kv_cache_read(const int8_t* nope_cache, const void* rope_cache, const vo
 }
 
 size_t pto_prompt_attention_workspace_bytes(int tq, int tk, int b, int hq, int hkv, int dv) {
-  if (tq < 0 || tk < 0 || b < 1 || hkv < 1 || hq < hkv || dv < 1 || static_cast<int64_t>(tq) * (hq / hkv) > INT_MAX - 512) return 0;
+  if (tq < 0 || tk < 0 || b < 1 || b > kPaSequences || hkv < 1 || hq < hkv || dv < 1 ||
+      static_cast<int64_t>(tq) * (hq / hkv) > INT_MAX - 512) {
+    return 0;
+  }
   return pa_ws(tq, tk, b, hq, hkv, dv).total;
 }
 
@@ -1372,7 +1377,7 @@ int pto_prompt_attention(const void* query, const void* key, const void* value, 
   PTO_REQUIRE(row_dtype(dtype), "dtype %d is neither bf16 nor f16", dtype);
   PTO_REQUIRE((dqk == 64 && dv == 64) || (dqk == 128 && dv == 128) || (dqk == 192 && dv == 128),
               "head dims %d / %d: 64 / 64, 128 / 128 or 192 / 128 expected", dqk, dv);
-  PTO_REQUIRE(tq >= 0 && tk >= 0 && b >= 0, "tq %d / tk %d / b %d", tq, tk, b);
+  PTO_REQUIRE(tq >= 0 && tk >= 0 && b >= 0 && b <= kPaSequences, "tq %d / tk %d / b %d", tq, tk, b);
   PTO_REQUIRE(hkv >= 1 && hq >= hkv && hq % hkv == 0, "%d query heads of %d key heads", hq, hkv);
   PTO_REQUIRE(softmax_scale > 0.f && softmax_scale <= 1e30f, "softmax_scale must be positive and finite");
   PTO_REQUIRE(strides != nullptr, "strides is null");

@@ -520,7 +520,7 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
   int64_t layout = 0, last = 0, rotary = 0;
   double eps = 0, amplitude = 0;
   if (n != 13 || !as_float(a[8], &eps) || !as_int(a[9], &layout) || !as_int(a[10], &last) || !as_int(a[11], &rotary) ||
-      !as_float(a[12], &amplitude) || eps < 0) {
+      !as_float(a[12], &amplitude) || !(eps >= 0)) {
     Py_RETURN_FALSE;
   }
   Call c;
@@ -633,7 +633,7 @@ PyObject* kv_cache_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* kv_cache_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
   PTO_GUARD_BEGIN
   int64_t bs = 0;
-  if (n != 10 || !as_int(a[7], &bs) || bs < 1 || (a[0] == Py_None) == (a[9] == Py_None)) Py_RETURN_FALSE;
+  if (n != 10 || !as_int(a[7], &bs) || bs < 1 || bs > INT32_MAX || (a[0] == Py_None) == (a[9] == Py_None)) Py_RETURN_FALSE;
   Call c;
   const at::Tensor* out = c.rows(a[5], 2);
   if (!c.ok()) Py_RETURN_FALSE;

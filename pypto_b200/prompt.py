@@ -270,7 +270,7 @@ def kv_cache_read(key_nope_2d, key_rope_2d, k_nope_scales, block_table, cu_seqle
     _need(cu.dtype == torch.int32 and cu.dim() == 1 and cu.shape[0] >= 1, "cu_seqlens: int32 [b + 1]")
     b = cu.shape[0] - 1
     _need(bt.dtype == torch.int32 and bt.dim() == 2 and bt.shape[0] == b, "block_table: int32 [b, max_blocks]")
-    _need(int(block_size) >= 1, "block_size must be positive")
+    _need(1 <= int(block_size) < 1 << 31, "block_size must be positive, and a 32-bit number")
     tensors = tensors + [out, bt, cu] + ([ro] if ro is not None else [])
     fs = None
     if first is not None:

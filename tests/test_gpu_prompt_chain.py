@@ -245,4 +245,6 @@ def test_c_entries_refuse_what_python_does_not_see():
         pto.prompt_attention(x, k.expand(9, 2, 64), k.expand(9, 2, 64), cu([4]), cu([9]), torch.empty_like(x))
     with pytest.raises(ValueError):
         pto.prompt_attention(x, k, k, cu([4]), cu([9]), torch.empty_like(x), math.inf)
+    with pytest.raises(ValueError):
+        pto.qk_norm_rope(x, None, torch.arange(4, device=DEV), pto.RotaryFrequencies(64), torch.empty_like(x), None, eps=math.nan)
     assert pto.launch_count() == before

@@ -35,6 +35,7 @@ def heads(**over):
     (dict(layout="sideways"), ValueError),
     (dict(rotary=10000.0), ValueError),
     (dict(eps=-1.0), ValueError),
+    (dict(eps=math.nan), ValueError),
     (dict(query=[1, 2]), TypeError),
 ])
 def test_norm_rope_refuses(over, exc):
@@ -89,6 +90,7 @@ def read(**over):
     (dict(key_rope_out=torch.zeros(4, 64, dtype=BF)), ValueError),
     (dict(key_nope_out=torch.zeros(5, 512, dtype=torch.float16)), ValueError),
     (dict(block_size=0), ValueError),
+    (dict(block_size=(1 << 32) + 1), ValueError),
     (dict(first=torch.zeros(3, dtype=torch.int32)), ValueError),
 ])
 def test_cache_read_refuses(over, exc):
@@ -138,6 +140,7 @@ def test_prompt_attention_workspace():
     assert 0 < one < (1 << 20) + 8 * 148 * 8 * 130 * 4
     assert lib.pto_prompt_attention_workspace_bytes(1 << 17, 1 << 17, 4, 128, 8, 128) < 200 << 20
     assert lib.pto_prompt_attention_workspace_bytes(1, 1, 0, 1, 1, 64) == 0
+    assert lib.pto_prompt_attention_workspace_bytes(1 << 30, 1, (1 << 31) - 1, 1, 1, 64) == 0  # more sequences than tiles are counted for
 
 
 def test_c_entries_refuse_before_any_cuda_call():
