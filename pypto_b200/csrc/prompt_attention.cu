@@ -64,7 +64,11 @@ struct Ctl {
   int odd[2];  // values that are not finite were taken out of an item's tiles
   uint32_t tmem;
   int expired;
-  float2 xch[128];  // maximum and sum of stream 1
+  PaHead head;
+  union {  // a table of a tile a lane is in the loader's registers before the first item is known to anyone
+    float2 xch[128];  // maximum and sum of stream 1
+    PaTile tile[32];
+  };
 };
 static_assert(sizeof(Ctl) <= 2048, "control block");
 constexpr int kSmem = 1024 + 14 * kBox + 2048;
@@ -360,8 +364,8 @@ __global__ void __launch_bounds__(1024) pa_plan_kernel(const PaParams p, int cta
 }
 
 // Item number w of a table: sets of key heads one after the other, in each the pieces of all tiles with the set's heads side by side.
-// Called by a converged warp.
-__device__ __forceinline__ Item find_item(const PaParams& p, const PaTile* tile, int tiles, int pieces, long long w) {
+// Called by a converged warp; `own`: the lane's tile of a table of at most 32.
+__device__ __forceinline__ Item find_item(const PaParams& p, const PaTile* tile, const PaTile& own, int tiles, int pieces, long long w) {
   Item it = {};
   if (w >= static_cast<long long>(pieces) * p.hkv) return it;
   const unsigned per_set = static_cast<unsigned>(pieces) * p.head_set;  // (pieces * heads: the host side refuses 2^31)
@@ -380,8 +384,8 @@ __device__ __forceinline__ Item find_item(const PaParams& p, const PaTile* tile,
     lo += last * step;
     n = min(step, n - last * step);
   }
-  PaTile t = {};
-  if (lane < n) t = tile[lo + lane];
+  PaTile t = own;
+  if (tiles > 32 && lane < n) t = tile[lo + lane];
   const int at = 31 - __clz(__ballot_sync(0xffffffffu, lane < n && t.piece <= which));
   t.q0 = __shfl_sync(0xffffffffu, t.q0, at);
   t.lq = __shfl_sync(0xffffffffu, t.lq, at);
@@ -458,12 +462,14 @@ __device__ __forceinline__ void role_load(const PaParams& p, const Ctx& x, const
   Ctl* c = x.c;
   const int lane = threadIdx.x & 31;
   const int tiles = head->tiles, pieces = head->pieces;
+  PaTile own = {};
+  if (lane < tiles && tiles <= 32) own = tile[lane];
   uint32_t pos = 0;
   long long w = blockIdx.x;
   for (uint32_t n_item = 0;; ++n_item) {
     const uint32_t buf = n_item & 1;
     wait_warp(c, c->mempty[buf], ((n_item >> 1) & 1) ^ 1, p.status, 80);
-    Item it = find_item(p, tile, tiles, pieces, w);
+    Item it = find_item(p, tile, own, tiles, pieces, w);
     if (*reinterpret_cast<volatile int*>(&c->expired)) it.valid = 0;
     it.valid = __shfl_sync(0xffffffffu, it.valid, 0);
     if (lane == 0) {
@@ -1070,7 +1076,8 @@ pa_kernel(const PaParams p, const __grid_constant__ CUtensorMap map_q, const __g
   uint8_t* base = smem_raw + (at - smem_u32(smem_raw));
   Ctl* c = reinterpret_cast<Ctl*>(base + 14 * kBox);
   const int warp = threadIdx.x >> 5;
-  if (threadIdx.x == 0) {
+  constexpr int kSetup = kThreads / 32 - 1;  // a warp that has nothing to look up for a short table: 900 cycles beside the first's loads
+  if (threadIdx.x == kSetup * 32) {
     for (int i = 0; i < C::kRing; ++i) {
       mbar_init(smem_u32(&c->full[i]), 1);
       mbar_init(smem_u32(&c->raw[i]), 1);
@@ -1095,7 +1102,7 @@ pa_kernel(const PaParams p, const __grid_constant__ CUtensorMap map_q, const __g
     c->expired = 0;
     fence_mbar_init();
   }
-  if (warp == 0) {
+  if (warp == kSetup) {
     tmem_alloc(smem_u32(&c->tmem), kTmemCols);
     tmem_relinquish();
   } else if (warp == 2 && p.tk > 0 && elect_one()) {
@@ -1107,7 +1114,13 @@ pa_kernel(const PaParams p, const __grid_constant__ CUtensorMap map_q, const __g
   PaTile* tile = reinterpret_cast<PaTile*>(head + 1);
   if (p.self_plan) {
     // (scratch in the ring: the barrier at its end and the fence come before the first copy into it)
-    build_table(p, head, tile, reinterpret_cast<int*>(tile + p.max_tiles), reinterpret_cast<PlanScratch*>(base), gridDim.x);
+    const bool here = p.max_tiles <= 32;  // (in the workspace the merge alone reads it: 16 tokens x 8 heads 88.1 -> 87.5 us)
+    if (here) head = &c->head, tile = c->tile;
+    build_table(p, head, tile, nullptr, reinterpret_cast<PlanScratch*>(base), gridDim.x);
+    if (here && p.slots > 0 && blockIdx.x == 0 && warp == 0) {
+      if ((threadIdx.x & 31) < head->tiles) reinterpret_cast<PaTile*>(table + sizeof(PaHead))[threadIdx.x & 31] = tile[threadIdx.x & 31];
+      if (elect_one()) *reinterpret_cast<PaHead*>(table) = *head;
+    }
   } else {
     pdl_wait();
   }
@@ -1133,7 +1146,7 @@ pa_kernel(const PaParams p, const __grid_constant__ CUtensorMap map_q, const __g
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 0) {
+  if (warp == kSetup) {
     tc_fence_after();
     tmem_dealloc(c->tmem, kTmemCols);
   }
