@@ -6,7 +6,7 @@
 // steps of 64 keys. TMEM holds the scores of two steps of each stream, whose first half the probabilities overwrite as 16-bit
 // values (the A operand of the value product from there), and both outputs; the scores of step i + 2 follow the value product of
 // step i, so the softmax finds the next step's scores ready while the tensor pipe works on the ones before. Measured on 8192 tokens x
-// 32 heads on 8 key heads of 128, causal: 462 us, 1190 TFLOP/s (72 % of the GEMM's burst rate; under the power cap of a long run 541).
+// 32 heads on 8 key heads of 128, causal: 451 us, 1219 TFLOP/s (74 % of the GEMM's burst rate; under the power cap of a long run 530).
 // Steps of 128 keys in one buffer, probabilities handed over by halves: the pipe waits for the softmax and the softmax for it, 497;
 // scores and probabilities of 64 keys in columns of their own, two hand-overs a step: 505, where this had 485. What bounds it is shared
 // memory, which delivers 128 bytes a cycle: score products of 64 keys take 48 cycles instead of 32, and without any softmax at all
@@ -162,6 +162,11 @@ __device__ __forceinline__ void sequence(const PaParams& p, int i, int& q0, int&
   k0 = min(max(__ldg(p.cu_k + i), 0), p.tk);
   lk = min(max(__ldg(p.cu_k + i + 1), k0), p.tk) - k0;
 }
+__device__ __forceinline__ void check_sequence(const PaParams& p, int i, int q0, int lq, int k0, int lk) {
+  if (q0 != __ldg(p.cu_q + i) || q0 + lq != __ldg(p.cu_q + i + 1) || k0 != __ldg(p.cu_k + i) || k0 + lk != __ldg(p.cu_k + i + 1)) {
+    set_status(p.status, PTO_ST_BAD_PAGE, i, 73);
+  }
+}
 __device__ __forceinline__ int tile_keys(const PaParams& p, const PaTile& t) {  // key tiles
   const int rows = min(kPaRows, t.lq * p.group - t.row0);
   const int keys = p.causal ? min(max(t.lk - t.lq + 1 + row_token(p, t.row0 + rows - 1), 0), t.lk) : t.lk;
@@ -190,9 +195,7 @@ __device__ void build_table(const PaParams& p, PaHead* head, PaTile* tile, int* 
     if (i < p.b) {
       int q0, lq, k0, lk;
       sequence(p, i, q0, lq, k0, lk);
-      if (q0 != __ldg(p.cu_q + i) || q0 + lq != __ldg(p.cu_q + i + 1) || k0 != __ldg(p.cu_k + i) || k0 + lk != __ldg(p.cu_k + i + 1)) {
-        set_status(p.status, PTO_ST_BAD_PAGE, i, 73);
-      }
+      check_sequence(p, i, q0, lq, k0, lk);
       count = static_cast<int>((static_cast<long long>(lq) * p.group + kPaRows - 1) / kPaRows);
     }
     int all;
@@ -355,6 +358,47 @@ __device__ void build_table(const PaParams& p, PaHead* head, PaTile* tile, int* 
   __syncthreads();
 }
 
+// The same for a table of at most 32 tiles that cannot be in pieces, by one warp without a barrier. (17 tokens x 8 heads: 10.2 us with the block's,
+// 8.8 with this.) `mark`: 32 ints.
+__device__ __forceinline__ void build_short_table(const PaParams& p, PaHead* head, PaTile* tile, int* mark) {
+  const int lane = threadIdx.x & 31;
+  PaTile x = {};
+  int count = 0;
+  mark[lane] = 0;
+  if (lane < p.b) {  // (b is at most max_tiles)
+    sequence(p, lane, x.q0, x.lq, x.k0, x.lk);
+    check_sequence(p, lane, x.q0, x.lq, x.k0, x.lk);
+    count = (x.lq * p.group + kPaRows - 1) / kPaRows;
+  }
+  const int end = warp_inclusive(count);
+  const int total = min(__shfl_sync(0xffffffffu, end, 31), p.max_tiles), first = end - count;
+  __syncwarp();
+  if (count > 0 && first < 32) mark[first] = lane;
+  __syncwarp();
+  int of = mark[lane];  // the tile's sequence: the last one that begins at or before it
+#pragma unroll
+  for (int o = 1; o < 32; o *= 2) {
+    const int y = __shfl_up_sync(0xffffffffu, of, o);
+    if (lane >= o) of = max(of, y);
+  }
+  x.row0 = (lane - __shfl_sync(0xffffffffu, first, of)) * kPaRows;
+  x.q0 = __shfl_sync(0xffffffffu, x.q0, of);
+  x.lq = __shfl_sync(0xffffffffu, x.lq, of);
+  x.k0 = __shfl_sync(0xffffffffu, x.k0, of);
+  x.lk = __shfl_sync(0xffffffffu, x.lk, of);
+  const int n = lane < total ? tile_keys(p, x) : -1;
+  int rank = 0;
+  for (int t = 0; t < total; ++t) {
+    const int k = __shfl_sync(0xffffffffu, n, t);
+    rank += k > n || (k == n && t < lane);
+  }
+  x.pieces = 1;
+  x.piece = rank;
+  x.slot = -1;
+  if (lane < total) tile[rank] = x;
+  if (lane == 0) *head = PaHead{total, total, 0, 0};
+}
+
 __global__ void __launch_bounds__(1024) pa_plan_kernel(const PaParams p, int ctas) {
   __shared__ PlanScratch s;
   pdl_trigger();
@@ -456,7 +500,7 @@ __device__ __forceinline__ int item_steps(const Item& it, int s) {
 }
 
 // K and V tiles through the ring, and the items
-template <typename C>
+template <typename C, bool kOwnTable>
 __device__ __forceinline__ void role_load(const PaParams& p, const Ctx& x, const CUtensorMap* mk, const CUtensorMap* mv, PaHead* head,
                                           const PaTile* tile) {
   Ctl* c = x.c;
@@ -478,7 +522,7 @@ __device__ __forceinline__ void role_load(const PaParams& p, const Ctx& x, const
     }
     if (!it.valid) break;
     int next = 0;
-    if (lane == 0 && !p.self_plan) next = atomicAdd(&head->next, 1);  // (its answer is due at the end of the item)
+    if (lane == 0 && !kOwnTable) next = atomicAdd(&head->next, 1);  // (its answer is due at the end of the item)
     auto load = [&](int slots, const CUtensorMap* map, int key_tile, bool edge) {
       for (int i = 0; i < slots; ++i, ++pos) {
         uint32_t slot, phase;
@@ -517,7 +561,7 @@ __device__ __forceinline__ void role_load(const PaParams& p, const Ctx& x, const
         if (k + 1 < n1) key(1, k + 1);
       }
     }
-    w = p.self_plan ? w + gridDim.x : static_cast<long long>(gridDim.x) + __shfl_sync(0xffffffffu, next, 0);
+    w = kOwnTable ? w + gridDim.x : static_cast<long long>(gridDim.x) + __shfl_sync(0xffffffffu, next, 0);
   }
   if (*reinterpret_cast<volatile int*>(&c->expired)) {  // copies in flight arrive before the CTA ends
     const long long t0 = clock64();
@@ -1066,7 +1110,9 @@ __device__ __forceinline__ void role_softmax(const PaParams& p, const Ctx& x, in
   }
 }
 
-template <int DQK, int DV, bool F16>
+// kOwnTable: every CTA builds the table. (Two kernels: with that code in the other's too, 4095 tokens x 128 heads of 192 took 416 us, not 371,
+// and 8192 x 32 of 128 465, not 451.)
+template <int DQK, int DV, bool F16, bool kOwnTable>
 __global__ void __launch_bounds__(kThreads, 1)
 pa_kernel(const PaParams p, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
           const __grid_constant__ CUtensorMap map_v) {
@@ -1109,14 +1155,18 @@ pa_kernel(const PaParams p, const __grid_constant__ CUtensorMap map_q, const __g
     tma_prefetch_desc(&map_k);
     tma_prefetch_desc(&map_v);
   }
-  uint8_t* table = p.tables + (p.self_plan ? blockIdx.x * p.table_stride : 0);
+  uint8_t* table = p.tables + (kOwnTable ? blockIdx.x * p.table_stride : 0);
   PaHead* head = reinterpret_cast<PaHead*>(table);
   PaTile* tile = reinterpret_cast<PaTile*>(head + 1);
-  if (p.self_plan) {
+  if constexpr (kOwnTable) {
     // (scratch in the ring: the barrier at its end and the fence come before the first copy into it)
     const bool here = p.max_tiles <= 32;  // (in the workspace the merge alone reads it: 16 tokens x 8 heads 88.1 -> 87.5 us)
     if (here) head = &c->head, tile = c->tile;
-    build_table(p, head, tile, nullptr, reinterpret_cast<PlanScratch*>(base), gridDim.x);
+    if (here && p.slots == 0) {
+      if (warp == 0) build_short_table(p, head, tile, reinterpret_cast<int*>(base));
+    } else {
+      build_table(p, head, tile, nullptr, reinterpret_cast<PlanScratch*>(base), gridDim.x);
+    }
     if (here && p.slots > 0 && blockIdx.x == 0 && warp == 0) {
       if ((threadIdx.x & 31) < head->tiles) reinterpret_cast<PaTile*>(table + sizeof(PaHead))[threadIdx.x & 31] = tile[threadIdx.x & 31];
       if (elect_one()) *reinterpret_cast<PaHead*>(table) = *head;
@@ -1138,7 +1188,7 @@ pa_kernel(const PaParams p, const __grid_constant__ CUtensorMap map_q, const __g
         else role_mma<C, DQK, DV, 1>(p, x);
       }
       __syncwarp();
-    } else if (warp == 2) role_load<C>(p, x, &map_k, &map_v, head, tile);
+    } else if (warp == 2) role_load<C, kOwnTable>(p, x, &map_k, &map_v, head, tile);
     else role_queries<C, DQK, DV, F16>(p, x, &map_q);
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
@@ -1220,7 +1270,8 @@ __global__ void __launch_bounds__(256) pa_merge_kernel(const PaParams p) {
 
 template <int DQK, int DV, bool F16>
 cudaError_t launch(const PaParams& p, const void* tmap_q, const void* tmap_k, const void* tmap_v, int ctas, cudaStream_t stream) {
-  cudaError_t e = cudaFuncSetAttribute(pa_kernel<DQK, DV, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  const auto kernel = p.self_plan ? pa_kernel<DQK, DV, F16, true> : pa_kernel<DQK, DV, F16, false>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) return e;
   if (!p.self_plan) {
     pa_plan_kernel<<<1, p.max_tiles <= kPaSmallTiles ? kPaSmallTiles : 1024, 0, stream>>>(p, ctas);
@@ -1228,7 +1279,7 @@ cudaError_t launch(const PaParams& p, const void* tmap_q, const void* tmap_k, co
     if (e != cudaSuccess) return e;
     count_launch();
   }
-  e = launch_maybe_pdl(pa_kernel<DQK, DV, F16>, dim3(ctas), dim3(kThreads), kSmem, stream, !p.self_plan, p,
+  e = launch_maybe_pdl(kernel, dim3(ctas), dim3(kThreads), kSmem, stream, !p.self_plan, p,
                        *reinterpret_cast<const CUtensorMap*>(tmap_q), *reinterpret_cast<const CUtensorMap*>(tmap_k), *reinterpret_cast<const CUtensorMap*>(tmap_v));
   if (e != cudaSuccess) return e;
   count_launch();
