@@ -126,6 +126,8 @@ def test_prompts(ql, kl, hq, hkv, dqk, dv, dtype):
     ([1] * 300, list(range(1, 301)), 4, 1, 128, 128, BF, True),
     ([1000, 3000, 2000] * 2, [1000, 3000, 2000] * 2, 16, 8, 64, 64, F16, True),
     ([1], [40000], 1, 1, 192, 128, F16, False),
+    ([0, 3, 0, 0, 1, 9, 2, 0] * 3 + [4] * 7, [0, 9, 5, 0, 1, 2, 16, 0] * 3 + [5, 4, 0, 8, 30, 4, 7], 2, 1, 64, 64, BF, True),  # 31 short ones
+    ([0, 0, 1200, 0, 700, 0], [3, 0, 400, 0, 90, 0], 4, 1, 128, 128, F16, False),  # row tiles of two sequences between empty ones
 ], ids=lambda x: str(x)[:24])
 def test_shapes(ql, kl, hq, hkv, dqk, dv, dtype, causal):
     run(ql, kl, hq, hkv, dqk, dv, dtype, causal)
