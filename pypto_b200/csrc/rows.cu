@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(kWarps * 32, kNorm ? 6 : 8) norm_rope_kernel(c
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
       mul[e] *= mine_w[e];
-      oth[e] *= other_w[kHalf ? e : e ^ 1];
+      if (rotated) oth[e] *= other_w[kHalf ? e : e ^ 1];
     }
   }
   const float inv_d = 1.f / static_cast<float>(s.d);
@@ -171,6 +171,12 @@ __global__ void __launch_bounds__(kWarps * 32, kNorm ? 6 : 8) norm_rope_kernel(c
 #pragma unroll
         for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
         for (int o = s.lanes >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        // a dim that has no pair takes nothing of its neighbour (inf * 0 is not 0); in halves it is its own, and what an infinity is
+        // divided by is one
+        if (!kHalf && !rotated && !(ss < INFINITY)) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = x[e] * mul[e];
+        }
         const float inv = rsqrtf(fmaf(ss, inv_d, p.eps));
 #pragma unroll
         for (int e = 0; e < 8; ++e) y[e] *= inv;
