@@ -45,6 +45,10 @@ struct Cfg {
 // Of eight pairs of probabilities, those whose exponentials the FMA pipe computes (8192 tokens, 0 to 3 of eight: 480, 462, 469, 472 us)
 constexpr int kFmaPairs = 1;
 constexpr float kLag = 8.f;  // a maximum is raised, and the output rescaled, once it is 2^8 behind
+// A row's exponents are taken relative to its maximum's, rounded to fp32: fma(score, scale, -fl(maximum * scale)), exact but for a
+// factor of 2^(up to half a step of the maximum's) in all of the row. From this exponent on that would be more than 2^(1/2), and soon
+// more than fp32 or f16 probabilities hold: there the maximum is taken from the scores before they are scaled.
+constexpr float kFar = 0x1p24f;
 
 struct alignas(16) Item {
   int valid, dual;
@@ -881,6 +885,26 @@ __device__ __forceinline__ float to_float(uint16_t v) {
   else return __uint_as_float(static_cast<uint32_t>(v) << 16);
 }
 
+// `scale`: of an exponent of 2
+__device__ __forceinline__ bool is_far(float m, float scale) { return m != -INFINITY && fabsf(m * scale) >= kFar; }
+// What probabilities relative to a maximum m weigh beside those relative to a larger one (or the same)
+__device__ __forceinline__ float weight_of(float m, float top, float scale) {
+  if (m == -INFINITY) return 0.f;
+  return ex2f(is_far(top, scale) ? (m - top) * scale : __fmul_rn(m, scale) - __fmul_rn(top, scale));
+}
+template <int DV>
+__device__ __forceinline__ void rescale(uint32_t t_o, float f) {
+#pragma unroll 1
+  for (int i = 0; i < DV / 32; ++i) {
+    uint32_t o[32];
+    tmem_ld_32x32b_x32(t_o + i * 32, o);
+    tc_wait_ld();
+#pragma unroll
+    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+    tmem_st_32x32b_x32(t_o + i * 32, o);
+  }
+}
+
 // 32 bytes of a row: one store where they lie on a 32-byte boundary
 __device__ __forceinline__ void store32(void* dst, const uint32_t (&w)[8], bool wide) {
   if (wide) {
@@ -914,7 +938,8 @@ __device__ __forceinline__ void role_softmax(const PaParams& p, const Ctx& x, in
     const int limit = row_limit(p, it, mine ? row : it.rows - 1);
     const int sure = row_limit(p, it, it.dual ? 0 : s * 128);  // keys that all rows of the stream see
     float m = -INFINITY, l = 0.f;                              // maximum (of the scores as they are) and sum
-    for (int k = 0; k < n; ++k, ++ns) {
+    int k = 0;
+    for (; k < n; ++k, ++ns) {
       const uint32_t t_s = x.tmem + lanes + s * 128 + (ns & 1) * 64;
       wait_bar(c, sfull + (ns & 1) * 8, (ns >> 1) & 1, p.status, 93);
       __syncwarp();
@@ -949,26 +974,20 @@ __device__ __forceinline__ void role_softmax(const PaParams& p, const Ctx& x, in
       float t = top[C::kStep / 16 - 1];
       if (t == INFINITY) t = NAN;  // inf - inf: what the row comes to in any case
       if (k == 0) {
+        if (__any_sync(0xffffffffu, is_far(t, sl))) break;
         m = t;
       } else {
         // the first maximum mostly stays good enough: the output is rescaled when it is more than 2^8 behind
         const bool raise = m == -INFINITY ? t != m : !((t - m) * sl <= kLag);
         if (__any_sync(0xffffffffu, raise)) {
+          if (__any_sync(0xffffffffu, raise && is_far(t, sl))) break;
           const float f = raise ? (m == -INFINITY ? 0.f : ex2f((m - t) * sl)) : 1.f;
           m = raise ? t : m;
           l *= f;
           // the value product before (the one before that came ahead of these scores)
           wait_warp(c, c->pfree[s], (ns - 1) & 1, p.status, 94);
           tc_fence_after();
-#pragma unroll 1
-          for (int i = 0; i < DV / 32; ++i) {
-            uint32_t o[32];
-            tmem_ld_32x32b_x32(t_o + i * 32, o);
-            tc_wait_ld();
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-            tmem_st_32x32b_x32(t_o + i * 32, o);
-          }
+          rescale<DV>(t_o, f);
         }
       }
       const float2 shift = both(C::kBias - (m == -INFINITY ? 0.f : m * sl));
@@ -998,6 +1017,59 @@ __device__ __forceinline__ void role_softmax(const PaParams& p, const Ctx& x, in
       if (lane == 0) mbar_arrive(pfull + (ns & 1) * 8);
       l += (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
     }
+    // The rest of an item in which a row of the warp has a maximum far from zero: the same steps, short rather than fast
+    for (bool far = false; k < n; ++k, ++ns) {
+      const uint32_t t_s = x.tmem + lanes + s * 128 + (ns & 1) * 64;
+      wait_bar(c, sfull + (ns & 1) * 8, (ns >> 1) & 1, p.status, 93);
+      __syncwarp();
+      tc_fence_after();
+      const int left = limit - (key0 + k * C::kStep);
+      float t = -INFINITY;
+#pragma unroll 1
+      for (int h = 0; h < C::kStep / 32; ++h) {
+        uint32_t o[32];
+        tmem_ld_32x32b_x32(t_s + 32 * h, o);
+        tc_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) t = max3(t, t, 32 * h + i < left ? __uint_as_float(o[i]) : -INFINITY);
+      }
+      if (t == INFINITY) t = NAN;
+      const bool raise = m == -INFINITY ? t != m : !((t - m) * sl <= kLag);
+      if (__any_sync(0xffffffffu, raise)) {
+        const float f = raise ? (m == -INFINITY ? 0.f : ex2f((m - t) * sl)) : 1.f;
+        m = raise ? t : m;
+        l *= f;
+        far = raise ? is_far(m, sl) : far;
+        if (k > 0) {
+          wait_warp(c, c->pfree[s], (ns - 1) & 1, p.status, 94);
+          tc_fence_after();
+          rescale<DV>(t_o, f);
+        }
+      }
+      const float from = far ? m : 0.f, shift = C::kBias - (far || m == -INFINITY ? 0.f : m * sl);
+#pragma unroll 1
+      for (int h = 0; h < C::kStep / 32; ++h) {
+        uint32_t o[32], w[16];
+        tmem_ld_32x32b_x32(t_s + 32 * h, o);
+        tc_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float y[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int at = 2 * i + j;
+            y[j] = 32 * h + at < left ? ex2f(fmaf(__uint_as_float(o[at]) - from, sl, shift)) : 0.f;
+            l += y[j];
+          }
+          w[i] = pack16<F16>(y[0], y[1]);
+        }
+        tmem_st_32x32b_x16(t_s + h * 16, w);
+      }
+      tc_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(pfull + (ns & 1) * 8);
+    }
 
     // ---- the item's output
     if (n > 0) {
@@ -1005,10 +1077,9 @@ __device__ __forceinline__ void role_softmax(const PaParams& p, const Ctx& x, in
       ++no;
       tc_fence_after();
     }
-    const float e = m * sl;  // exponent of the maximum
     if (it.dual && s == 1) {
       wait_warp(c, c->xempty, (nx & 1) ^ 1, p.status, 97);
-      c->xch[r] = make_float2(n > 0 ? e : -INFINITY, l);
+      c->xch[r] = make_float2(m, l);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&c->xfull));
@@ -1018,7 +1089,7 @@ __device__ __forceinline__ void role_softmax(const PaParams& p, const Ctx& x, in
       if (lane == 0) mbar_arrive(smem_u32(&c->mempty[buf]));
       continue;
     }
-    float f0 = 1.f, f1 = 0.f, top = n > 0 ? e : -INFINITY, all = l;
+    float f0 = 1.f, f1 = 0.f, top = m, all = l;
     bool two = false;
     if (it.dual) {
       wait_warp(c, c->xfull, nx & 1, p.status, 98);
@@ -1027,8 +1098,8 @@ __device__ __forceinline__ void role_softmax(const PaParams& p, const Ctx& x, in
       two = it.end[1] > it.begin[1];
       if (two) {
         const float best = fmaxf(top, o.x);
-        f0 = top == -INFINITY ? 0.f : ex2f(top - best);
-        f1 = o.x == -INFINITY ? 0.f : ex2f(o.x - best);
+        f0 = weight_of(top, best, sl);
+        f1 = weight_of(o.x, best, sl);
         all = l * f0 + o.y * f1;
         top = best;
       }
@@ -1098,7 +1169,7 @@ __device__ __forceinline__ void role_softmax(const PaParams& p, const Ctx& x, in
       if (it.slot >= 0) {
         p.part_ml[static_cast<int64_t>(it.slot) * p.slot_rows + row] = make_float2(top, all);
       } else if (p.lse != nullptr) {
-        p.lse[static_cast<int64_t>(h) * p.tq + token] = all == 0.f ? -INFINITY : (top - C::kBias + log2f(all)) * kLn2;
+        p.lse[static_cast<int64_t>(h) * p.tq + token] = all == 0.f ? -INFINITY : (top * sl - C::kBias + log2f(all)) * kLn2;
       }
     }
     tc_fence_before();
@@ -1202,7 +1273,7 @@ pa_kernel(const PaParams p, const __grid_constant__ CUtensorMap map_q, const __g
   }
 }
 
-// Tiles in several pieces: their partial results, weighted by exp2(maximum - the largest maximum). A warp a row.
+// Tiles in several pieces: their partial results, weighted by 2^(maximum - the largest maximum). A warp a row.
 template <int DV, bool F16>
 __global__ void __launch_bounds__(256) pa_merge_kernel(const PaParams p) {
   constexpr int kPer = DV / 32;
@@ -1230,7 +1301,7 @@ __global__ void __launch_bounds__(256) pa_merge_kernel(const PaParams p) {
       for (int i0 = 0; i0 < t.pieces; i0 += 32) {
         float2 ml = own;
         if (i0 > 0) ml = i0 + lane < t.pieces ? p.part_ml[(slot + i0 + lane) * p.slot_rows + row] : make_float2(-INFINITY, 0.f);
-        const float weight = ml.x == -INFINITY ? 0.f : ex2f(ml.x - top);  // (0: it has seen no key)
+        const float weight = weight_of(ml.x, top, p.scale_log2);  // (0: it has seen no key)
         all += ml.x == -INFINITY ? 0.f : ml.y * weight;
         const int n = min(32, t.pieces - i0);
         const float* src = p.part_o + ((slot + i0) * p.slot_rows + row) * DV + lane * kPer;
@@ -1262,7 +1333,7 @@ __global__ void __launch_bounds__(256) pa_merge_kernel(const PaParams p) {
         *reinterpret_cast<uint32_t*>(dst) = pack16<F16>(y[0] * inv, y[1] * inv);
       }
       if (lane == 0 && p.lse != nullptr) {
-        p.lse[static_cast<int64_t>(h) * p.tq + t.q0 + tok] = all == 0.f ? -INFINITY : (top - Cfg<128, DV, F16>::kBias + log2f(all)) * kLn2;
+        p.lse[static_cast<int64_t>(h) * p.tq + t.q0 + tok] = all == 0.f ? -INFINITY : (top * p.scale_log2 - Cfg<128, DV, F16>::kBias + log2f(all)) * kLn2;
       }
     }
   }

@@ -41,7 +41,7 @@ struct PaParams {
   int self_plan;        // every CTA builds the table
   uint8_t* tables;      // PaHead, PaTile [max_tiles], int first [b + 1]; `table_stride` bytes a CTA
   int64_t table_stride;
-  float2* part_ml;      // [slot][slot_rows]: maximum (exponent of 2), sum
+  float2* part_ml;      // [slot][slot_rows]: maximum of the scores, sum
   float* part_o;        // [slot][slot_rows][dv]
   int slots;            // 0: no item can be in pieces
   int32_t* status;
