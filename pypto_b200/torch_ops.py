@@ -17,6 +17,7 @@ this implementation reads, so they are not part of the op schemas).
 """
 from __future__ import annotations
 
+import inspect
 from typing import Optional
 
 import torch
@@ -25,6 +26,10 @@ from torch import Tensor
 from . import ops, prompt
 
 _NS = "pypto_b200"
+
+
+def _no_result(*args, **kwargs) -> None:
+    return None
 
 
 @torch.library.custom_op(f"{_NS}::lightning_indexer_decode", mutates_args=("topk_res",))
@@ -137,7 +142,31 @@ def qk_norm_rope(query: Tensor, key: Optional[Tensor], positions: Tensor, turns:
                         query_weight=query_weight, key_weight=key_weight, eps=eps, layout=layout, rope_last=rope_last)
 
 
-@torch.library.custom_op(f"{_NS}::kv_cache_write", mutates_args=("key_nope_2d", "key_rope_2d", "k_nope_scales", "packed_kv_cache"))
+_fragment = torch.library.Library(_NS, "FRAGMENT")
+
+
+def _op_with_optional_buffers(*written):
+    """As `custom_op`, for operators whose last arguments are written where they are given: the dispatcher leaves out trailing
+    arguments that are their defaults, and `custom_op` then looks for the buffers behind the end of what it got."""
+    def register(fn):
+        name, schema = fn.__name__, torch.library.infer_schema(fn, mutates_args=written)
+        signature = inspect.signature(fn)
+
+        def impl(*args, **kwargs):
+            fn(*args, **kwargs)
+            given = signature.bind(*args, **kwargs).arguments
+            for w in written:
+                if given.get(w) is not None:
+                    torch.autograd.graph.increment_version(given[w])
+
+        _fragment.define(f"{name}{schema}", tags=torch.Tag.pt2_compliant_tag)
+        _fragment.impl(name, impl, "CompositeExplicitAutograd")
+        torch.library.register_fake(f"{_NS}::{name}", _no_result, lib=_fragment)
+        return getattr(getattr(torch.ops, _NS), name)
+    return register
+
+
+@_op_with_optional_buffers("key_nope_2d", "key_rope_2d", "k_nope_scales", "packed_kv_cache")
 def kv_cache_write(key_nope: Tensor, key_rope: Optional[Tensor], cache_index: Tensor, key_nope_2d: Optional[Tensor],
                    key_rope_2d: Optional[Tensor], k_nope_scales: Optional[Tensor], packed_kv_cache: Optional[Tensor] = None) -> None:
     prompt.kv_cache_write(key_nope, key_rope, cache_index, key_nope_2d, key_rope_2d, k_nope_scales, packed_kv_cache=packed_kv_cache)
@@ -151,18 +180,15 @@ def kv_cache_read(key_nope_2d: Optional[Tensor], key_rope_2d: Optional[Tensor], 
                          first=first, packed_kv_cache=packed_kv_cache)
 
 
-@torch.library.custom_op(f"{_NS}::prompt_attention", mutates_args=("attention_out", "lse_out"))
+@_op_with_optional_buffers("attention_out", "lse_out")
 def prompt_attention(query: Tensor, key: Tensor, value: Tensor, cu_seqlens_q: Tensor, cu_seqlens_k: Tensor, attention_out: Tensor,
                      softmax_scale: float, causal: bool = True, lse_out: Optional[Tensor] = None) -> None:
     prompt.prompt_attention(query, key, value, cu_seqlens_q, cu_seqlens_k, attention_out, softmax_scale, causal=causal, lse_out=lse_out)
-
-
-def _no_result(*args, **kwargs) -> None:
-    return None
 
 
 OPS = (lightning_indexer_decode, sparse_flash_attention_quant, sparse_attention_antiquant,
        decode_indexer_attention_quant, lightning_indexer_topk_nonquant, decode_indexer_attention,
        mla_indexer_prolog_quant, mla_indexer_prolog, qk_norm_rope, kv_cache_write, kv_cache_read, prompt_attention)
 for _op in OPS:
-    _op.register_fake(_no_result)
+    if isinstance(_op, torch.library.CustomOpDef):
+        _op.register_fake(_no_result)
