@@ -133,13 +133,14 @@ def mla_indexer_prolog(token_x: Tensor, w_dq: Tensor, w_uq_qr: Tensor, w_uk: Ten
 
 
 @torch.library.custom_op(f"{_NS}::qk_norm_rope", mutates_args=("query_out", "key_out"))
-def qk_norm_rope(query: Tensor, key: Optional[Tensor], positions: Tensor, turns: Tensor, query_out: Tensor,
+def qk_norm_rope(query: Tensor, key: Optional[Tensor], positions: Optional[Tensor], turns: Optional[Tensor], query_out: Tensor,
                  key_out: Optional[Tensor], query_weight: Optional[Tensor], key_weight: Optional[Tensor], amplitude: float = 1.0,
                  eps: float = 1e-6, layout: str = "half", rope_last: bool = False) -> None:
-    """`turns`, `amplitude`: those of a `RotaryFrequencies`. Outputs apart from the inputs (an input written in place has no place in a
-    schema that names what is written)."""
-    prompt.qk_norm_rope(query, key, positions, prompt.RotaryFrequencies.of(turns, amplitude), query_out, key_out,
-                        query_weight=query_weight, key_weight=key_weight, eps=eps, layout=layout, rope_last=rope_last)
+    """`turns`, `amplitude`: those of a `RotaryFrequencies`; without turns the norm alone. Outputs apart from the inputs (an input
+    written in place has no place in a schema that names what is written)."""
+    rotary = None if turns is None else prompt.RotaryFrequencies.of(turns, amplitude)
+    prompt.qk_norm_rope(query, key, positions, rotary, query_out, key_out, query_weight=query_weight, key_weight=key_weight, eps=eps,
+                        layout=layout, rope_last=rope_last)
 
 
 _fragment = torch.library.Library(_NS, "FRAGMENT")
@@ -182,7 +183,7 @@ def kv_cache_read(key_nope_2d: Optional[Tensor], key_rope_2d: Optional[Tensor], 
 
 @_op_with_optional_buffers("attention_out", "lse_out")
 def prompt_attention(query: Tensor, key: Tensor, value: Tensor, cu_seqlens_q: Tensor, cu_seqlens_k: Tensor, attention_out: Tensor,
-                     softmax_scale: float, causal: bool = True, lse_out: Optional[Tensor] = None) -> None:
+                     softmax_scale: Optional[float] = None, causal: bool = True, lse_out: Optional[Tensor] = None) -> None:
     prompt.prompt_attention(query, key, value, cu_seqlens_q, cu_seqlens_k, attention_out, softmax_scale, causal=causal, lse_out=lse_out)
 
 

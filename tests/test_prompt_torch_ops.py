@@ -90,3 +90,44 @@ def test_compiled_calls_without_optional_buffers(backend):
     write(*rows[:3], None, packed)
     for a, b in zip((*rows[3], want_packed), (*again, packed)):
         assert torch.equal(a, b) and bool(a.any())
+
+
+def _norm_alone(x, w, out):
+    _ns().qk_norm_rope(x, None, None, None, out, None, w, None)
+
+
+def _default_scale(x, cu, out):
+    _ns().prompt_attention(x, x, x, cu, cu, out)
+
+
+def test_norm_alone_and_the_default_scale_trace_without_a_device():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        x = torch.empty(5, 4, 128, dtype=BF)
+        _norm_alone(x, torch.empty(128, dtype=BF), torch.empty_like(x))
+        _default_scale(x, torch.empty(2, dtype=torch.int32), torch.empty_like(x))
+
+
+def test_norm_alone_and_the_default_scale_reach_the_operators_checks():
+    x, cu = _inputs("cpu")
+    with pytest.raises(RuntimeError, match="device"):
+        _norm_alone(x, torch.ones(128, dtype=BF), torch.empty_like(x))
+    with pytest.raises(RuntimeError, match="device"):
+        _default_scale(x, cu, torch.empty_like(x))
+    turns = pto.RotaryFrequencies(64, device="cpu").turns
+    with pytest.raises(TypeError, match="positions"):  # a rotation without positions
+        _ns().qk_norm_rope(x, None, None, turns, torch.empty_like(x), None, None, None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+def test_compiled_norm_alone_and_default_scale(backend):
+    x, cu = _inputs("cuda")
+    w, want, got = x[0, 0].clone(), torch.zeros_like(x), torch.zeros_like(x)
+    pto.qk_norm_rope(x, None, None, None, want, None, query_weight=w)
+    torch.compile(_norm_alone, backend=backend, fullgraph=True)(x, w, got)
+    assert torch.equal(want, got) and bool(got.any())
+    pto.prompt_attention(x, x, x, cu, cu, want)
+    torch.compile(_default_scale, backend=backend, fullgraph=True)(x, cu, got)
+    assert torch.equal(want, got)
