@@ -35,6 +35,11 @@ struct Cfg {
   static constexpr int kQ = DQK / 64 * kBox;
   static constexpr int kRing = (14 * kBox - 2 * kQ) / kSlot;  // 12, 5, 8 slots
   static constexpr int kK = DQK / 64 / kSlotBoxes, kV = DV / 64 / kSlotBoxes;  // slots of a K and of a V tile
+  // From the slot that a stream waited for last to its next one: at most a K and a V tile of the other stream's between them. That is
+  // within a lap, so what the loader had to see given back before it filled the last one covers the next one's use two laps ago, and
+  // the barriers' parities, which tell even laps from odd ones, are unambiguous. (An item's first slot comes right behind the whole
+  // item before, which the loader had issued when it gave out the item.)
+  static_assert(kK + kV + 1 <= kRing, "a stream's next slot is more than a lap away");
   static constexpr int kStep = 64, kSteps = kPaKeys / kStep;  // keys of a step, steps of a tile
   static constexpr uint32_t kColO = 256;                      // first column of the outputs, behind two streams' two buffers of scores
   static constexpr uint32_t kFmt = F16 ? 0u : kABFmtBF16;
