@@ -375,7 +375,8 @@ int pto_qk_norm_rope(const void* query, const void* key, const void* positions, 
 
 /* Rows into the quantised paged caches, int8 with one scale per 128 dims (the prologs' arithmetic: q = rint(x * (127 / max)),
  * scale = 1 / (127 / max)), at row cache_index[i]; rope dims are copied. Index -1: a padding row, not written; another index outside
- * the cache sets PTO_ST_BAD_PAGE and is skipped. The indices of a call are distinct. Groups below 2^-120 are stored as zeros.
+ * the cache sets PTO_ST_BAD_PAGE and is skipped. The indices of a call are distinct. Groups below 2^-120 are stored as zeros. f16
+ * scales hold groups whose largest magnitude is between 8e-3 and 8e6 to their precision; below they lose bits, above they are infinite.
  *   key_nope [t, width] (row stride ld_nope), width a multiple of 128; key_rope bf16 [t, 64] or null (then rope_cache is not written)
  *   split caches: nope_cache int8 [cache_rows, width], rope_cache bf16 [cache_rows, 64], scales f32 or f16 [cache_rows, width/128]
  *   packed_cache int8 [cache_rows, 656] (width 512 with rope); either form may be null

@@ -6,13 +6,17 @@
 // steps of 64 keys. TMEM holds the scores of two steps of each stream, whose first half the probabilities overwrite as 16-bit
 // values (the A operand of the value product from there), and both outputs; the scores of step i + 2 follow the value product of
 // step i, so the softmax finds the next step's scores ready while the tensor pipe works on the ones before. Measured on 8192 tokens x
-// 32 heads on 8 key heads of 128, causal: 451 us, 1219 TFLOP/s (74 % of the GEMM's burst rate; under the power cap of a long run 530).
+// 32 heads on 8 key heads of 128, causal: 452 to 470 us, 1170 to 1216 TFLOP/s (71 to 73 % of the GEMM's burst rate; under the power cap
+// of a long run 521).
 // Steps of 128 keys in one buffer, probabilities handed over by halves: the pipe waits for the softmax and the softmax for it, 497;
 // scores and probabilities of 64 keys in columns of their own, two hand-overs a step: 505, where this had 485. What bounds it is shared
 // memory, which delivers 128 bytes a cycle: score products of 64 keys take 48 cycles instead of 32, and without any softmax at all
 // the kernel still takes 401 us.
 // An item of at most 128 rows (a few tokens, single ones) has one tile; both streams take it, each with half of the keys, and the
 // halves are merged at the end.
+// Scores, maxima, sums and outputs are fp32. Probabilities alone are rounded to the rows' type, since the value product takes 16-bit
+// operands; their sum is that of the unrounded ones. That adds a third to the error that rounding the output has in any case: bf16
+// 0.0020 of the outputs' size from the definition in 64 bits, where fp32 throughout and one rounding has 0.0015; f16 0.00029 for 0.00021.
 // Warps: 0 and 1 issue the MMAs of stream 0 and 1, 2 hands out items and loads K and V by TMA through a ring, 3 loads queries and
 // mends the value tiles at a mask's edge, 4-7 and 8-11 are the softmax of stream 0 and 1, one thread a row.
 #include "prompt_attention.cuh"

@@ -61,10 +61,11 @@ __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
 // y = x / sqrt(mean x^2 + eps) * w; of the rotated dims every pair (a, b) -> (a cos - b sin, a sin + b cos) with the angle
 // position * frequency. A frequency is held in turns a position as a 64-bit binary fraction: the product with the position, taken
 // mod 2^64, IS the fraction of a turn, exact at any position, where an angle in fp32 loses 1e-2 rad at 10^5. cos and sin of its
-// upper 32 bits are within 1e-7.
+// upper 32 bits are within 2.5e-7, times the amplitude: 9.4e-8 of the fraction's rounding to fp32 (half a step of 2^-24 of half a
+// turn), the rest the function's and the amplitude's.
 // A lane holds eight neighbouring dims of a head, a power of two of lanes a head, so sums and the other half of a pair travel by
 // shuffles. With weights, cosines and sines multiplied beforehand a dim costs four operations besides its conversions: the kernel with a
-// norm is bound by instructions (16384 tokens x 40 heads 78 us; with the products taken one by one 88, issue slots 76 % busy).
+// norm is bound by instructions (16384 tokens x 40 heads 78 us, issue slots 77 % busy; with the products taken one by one 88, 76 %).
 // A warp takes heads of ONE token: its lanes' factors are computed once and stay in registers. With few tokens the heads of one are
 // shared out over as many warps as fill the SMs.
 template <int kLayout>

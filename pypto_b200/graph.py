@@ -6,7 +6,8 @@ An operator call is capturable as it is: it allocates nothing once its workspace
 stream exists, never synchronises, and reads the sequence lengths on the device. `CapturedCall` does the
 one warm-up call on the capture stream (which creates that workspace), records the call into a
 `torch.cuda.CUDAGraph` and replays it; the tensors passed in are the graph's static inputs and outputs:
-update them in place between replays.
+update them in place between replays. The warm-up is a call like any other: an operator that works in place
+(`qk_norm_rope` with its inputs as outputs) has changed them once by then, so fill them before the first replay.
 """
 from __future__ import annotations
 

@@ -209,9 +209,11 @@ def _cache_form(width, rope, key_nope_2d, key_rope_2d, k_nope_scales, packed_kv_
 
 def kv_cache_write(key_nope, key_rope, cache_index, key_nope_2d, key_rope_2d, k_nope_scales, *, packed_kv_cache=None):
     """Rows into the quantised paged caches at `cache_index` (int64 [t], distinct; -1: a padding row, not written): int8 with one
-    scale per 128 dims, the prologs' arithmetic; rope dims are copied.
+    scale per 128 dims, the prologs' arithmetic; rope dims are copied. float16 scales keep their precision for groups whose largest
+    magnitude lies between 8e-3 and 8e6; below they lose bits (under 4e-6 the group), above they are infinite.
 
-    key_nope [t, width], width a multiple of 128 (512: latent rows; 128 * hk: the keys or values of hk heads); key_rope bfloat16
+    key_nope [t, width], width a multiple of 128 (512: latent rows; 128 * hk: the keys or values of hk heads; two heads of 64 share a
+    group and its scale); key_rope bfloat16
     [t, 64] or None. Written in place: key_nope_2d int8 [rows, width], key_rope_2d bfloat16 [rows, 64] (None without key_rope),
     k_nope_scales float32 or float16 [rows, width/128], and / or `packed_kv_cache` int8 [rows, 656]: the caches that
     `sparse_flash_attention_quant_d/_p` and `sparse_attention_antiquant_d/_p` read. An index outside the cache is skipped and sets
@@ -291,6 +293,7 @@ def kv_cache_read(key_nope_2d, key_rope_2d, k_nope_scales, block_table, cu_seqle
 def prompt_attention(query, key, value, cu_seqlens_q, cu_seqlens_k, attention_out, softmax_scale=None, *, causal=True, lse_out=None):
     """Attention of packed sequences over all of their keys: token i of a sequence's lq sees keys j <= i + lk - lq of its lk (all of
     them with causal=False), so a chunk of a prompt comes with its earlier keys in front, and a single token with its whole context.
+    Keys and values lie packed, sequence behind sequence: what is in paged caches is read back first (`kv_cache_read`).
 
     query [tq, hq, dqk], key [tk, hkv, dqk], value [tk, hkv, dv], attention_out [tq, hq, dv]; (dqk, dv) (64, 64), (128, 128) or
     (192, 128) (the latent path after its up-projections); query head h reads key head h / (hq / hkv). cu_seqlens_q, cu_seqlens_k int32
